@@ -168,7 +168,7 @@ def prepare(case, seed):
         need = int((-(-(lengths + new) // page) + -lengths // page).sum())
         free = torch.randperm(2 * need + 50, generator=g, device="cuda").to(torch.int32)
         # some pages of the list are gone already, and a batch is padded to a few more tokens than it has
-        return {"case": case, "table": table, "free": free, "taken": torch.tensor([5, 0], dtype=torch.int32, device="cuda"),
+        return {"case": case, "table": table, "free": free, "taken": torch.tensor([5], dtype=torch.int32, device="cuda"),
                 "lengths": on_gpu(lengths), "new": on_gpu(new), "tokens": int(new.sum()) + 3}
     table, pages = _table(case, lengths + new, columns, g)
     request = np.repeat(np.arange(len(new)), new)
@@ -246,8 +246,7 @@ def _plain_slots(s):
     column = place.div(page, rounding_mode="floor")
     found = torch.where(inside & (column < W), table[r, column.clamp(max=W - 1)].long(), -1)
     slots = torch.where(found >= 0, found * page + place % page, -1)
-    lost = taken[1] + ends[-1] - (slots >= 0).sum()
-    return slots, (old + new).int(), torch.stack([(taken[0] + (b - a).sum()).clamp(max=F), lost]).int(), table
+    return slots, (old + new).int(), (taken + (b - a).sum()).int(), table
 
 
 def work(case):
