@@ -23,6 +23,13 @@ _i32p = C.POINTER(C.c_int32)
 _f64p = C.POINTER(C.c_double)
 _vp = C.c_void_p
 
+
+class PagedCache(C.Structure):
+    """``blk_paged_cache_t``."""
+    _fields_ = [("k", _vp), ("v", _vp), ("pages", C.c_int64), ("page_size", C.c_int64), ("heads", C.c_int64), ("head_dim", C.c_int64),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64), ("dtype", C.c_int)]
+
+
 # name -> (restype, argtypes); one entry per function declared in include/blkattn.h
 SIGNATURES = {
     "blk_last_error": (C.c_char_p, []),
@@ -51,6 +58,12 @@ SIGNATURES = {
     "blk_softmax_run": (C.c_int, [_vp, _vp, _vp, C.c_float, _vp]),
     "blk_softmax_backward_run": (C.c_int, [_vp, _vp, _vp, _vp, C.c_float, _vp]),
     "blk_softmax_noalloc": (C.c_int, [_vp, _vp, _i64p, _i64p, C.c_int64, C.c_int64, C.c_int, C.c_float, _vp]),
+    "blk_paged_slots": (C.c_int, [_vp, _vp, C.c_int64, _vp, C.c_int64, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64,
+                                  _vp, _vp, _vp]),
+    "blk_paged_append": (C.c_int, [C.POINTER(PagedCache), _vp, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64, _vp, C.c_int64, _vp]),
+    "blk_paged_attention_workspace": (C.c_int, [C.POINTER(PagedCache), C.c_int64, C.c_int64, C.c_int64, _i64p]),
+    "blk_paged_attention": (C.c_int, [C.POINTER(PagedCache), _vp, C.c_int64, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64, _vp,
+                                      C.c_int64, C.c_float, _vp, _vp, _vp, C.c_int64, _vp]),
     "blk_plan_destroy": (None, [_vp]),
     "blk_plan_extents": (C.c_int, [_vp, _i64p, _i64p, _i64p]),
     "blk_plan_offsets": (C.c_int, [_vp, _i64p, _i64p, _i64p]),

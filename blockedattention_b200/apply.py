@@ -197,6 +197,46 @@ def blockAttnScoresTokenMajor(q: torch.Tensor, k: torch.Tensor, nList, scale: fl
     return _ops.scores_token_major(q, k, nList, scale, out_dtype, softmax)
 
 
+def blockPagedSlots(lengths: torch.Tensor, newTokens: torch.Tensor, pageTable: torch.Tensor, freePages: torch.Tensor,
+                    taken: torch.Tensor, pageSize: int, tokens: int, *, advance: bool = False):
+    """Pages and slots for the new tokens of every request of a paged cache, worked out on the GPU.
+
+    Request r holds ``lengths[r]`` tokens and gets ``newTokens[r]``.  What they need beyond its ``ceil(lengths[r] /
+    pageSize)`` pages is taken from ``freePages``, from entry ``taken[0]`` on and request by request, and entered into
+    its row of ``pageTable -> (requests, columns)``, in place.  Returns ``(slots, lengths, taken)``: for each of the
+    new tokens, in the order of the requests, ``page * pageSize + place`` as int64 (``tokens`` entries, at
+    least as many as there are new tokens if none is to go without; -1 behind the last one, and for a token that finds no page
+    because the free ones are used up or its request's row is full); the requests' new lengths; and the
+    number of pages asked for so far (more than ``freePages`` has: they ran out).  ``advance=True`` writes these two into ``lengths`` and
+    ``taken`` themselves, for steps that are captured and replayed.  All index tensors but the slots are int32 on one GPU; nothing
+    is read by the host."""
+    return _ops.paged_slots(lengths, newTokens, pageTable, freePages, taken, pageSize, tokens, advance)
+
+
+def blockPagedAppend(k: torch.Tensor, v: torch.Tensor, kCache: torch.Tensor, vCache: torch.Tensor, slots: torch.Tensor) -> None:
+    """Writes new keys and values to their slots of a paged cache, in place: ``k, v -> (tokens, heads, d)``, token-major as
+    ``blockAttentionTokenMajor`` takes them, ``slots -> (tokens,)`` as ``blockPagedSlots`` gives them (no slot twice; those
+    outside the cache are passed over).  ``kCache, vCache -> (pages, heads, pageSize, d)`` of one shape and strides, rows
+    contiguous and 16-byte aligned; a cache kept as (pages, pageSize, heads, d) is given as its ``transpose(1, 2)``."""
+    _ops.paged_append(k, v, kCache, vCache, slots)
+
+
+def blockPagedAttention(q: torch.Tensor, kCache: torch.Tensor, vCache: torch.Tensor, pageTable: torch.Tensor,
+                        lengths: torch.Tensor, scale: float = 1.0, *, return_lse: bool = False):
+    """Attention of one new token per request over what a paged cache keeps: ``q -> (requests, heads, d)``, result of the
+    same shape, ``out[r, h] = softmax(scale * q[r, h] K^T) V`` over the first ``lengths[r]`` tokens of request r, whose
+    pages row r of ``pageTable`` names (both int32 on the GPU; nothing is read by the host).
+
+    ``kCache, vCache -> (pages, cache heads, pageSize, d)`` as for ``blockPagedAppend``; ``heads`` is a multiple of the cache's, and
+    that many consecutive heads of q share a head of the cache.  fp16, bf16 or fp32, ``d`` up to 256 in rows of whole 16
+    bytes, pages of any size.  Tokens on a table entry that is no page (-1: let go of, as by a sliding window) take no part;
+    a request without any gets zeros.  ``return_lse``: ``(out, lse)`` with each row's natural logarithm of
+    ``sum exp(scale * q K^T)`` (-inf without tokens), which is what joins the result with attention over other keys.
+    Forward only."""
+    run = _ops.paged_attention_lse if return_lse else _ops.paged_attention
+    return run(q, kCache, vCache, pageTable, lengths, scale)
+
+
 class _HostPipe:
     """Device-side staging of ``blockAttnScoresHost`` for one (lists, H, dtypes, device): a plan for a group of
     heads, two sets of device buffers and three streams (copy in, compute, copy out)."""

@@ -1046,3 +1046,207 @@ extern "C" int blk_softmax_backward_run(const blk_plan_t* p, const void* out, co
     if (e != cudaSuccess) return cuda_fail("softmax backward launch", e);
     return BLK_OK;
 }
+
+// ---- paged cache ---------------------------------------------------------------------------------------------
+namespace {
+
+int refused(const char* where, const char* what, int code = BLK_ERR_INVALID) {
+    blk_set_error(std::string(where) + ": " + what);
+    return code;
+}
+int64_t bytes_of(int dtype) { return dtype == BLK_F32 ? 4 : 2; }
+
+// Strides that no row uses (extents of one) are left out of every check.
+int check_paged_cache(const char* where, const blk_paged_cache_t* c) {
+    if (!c) return refused(where, "no cache");
+    if (c->dtype != BLK_F16 && c->dtype != BLK_BF16 && c->dtype != BLK_F32) return refused(where, "unknown dtype", BLK_ERR_UNSUPPORTED);
+    if (c->pages < 0 || c->pages > 0x7fffffffLL) return refused(where, "pages must be 0 to 2^31 - 1");
+    if (c->page_size < 1 || c->page_size > (1LL << 30)) return refused(where, "the page size must be 1 to 2^30 tokens");
+    if (c->heads < 1 || c->heads > 0xffffLL) return refused(where, "the cache must have 1 to 65535 heads");
+    if (c->head_dim < 1 || c->head_dim * bytes_of(c->dtype) % 16 || c->head_dim > 0xffffLL)
+        return refused(where, "rows (head_dim elements) must be multiples of 16 bytes", BLK_ERR_UNSUPPORTED);
+    if (c->pages > 0 && (!c->k || !c->v)) return refused(where, "null buffer");
+    const int64_t e = bytes_of(c->dtype);
+    if (!aligned16(c->k) || !aligned16(c->v) || (c->pages > 1 && c->page_stride * e % 16) || (c->heads > 1 && c->head_stride * e % 16) ||
+        (c->page_size > 1 && c->token_stride * e % 16))
+        return refused(where, "rows of the cache must start on 16-byte boundaries", BLK_ERR_UNALIGNED);
+    if ((c->pages > 1 && c->page_stride < 0) || (c->heads > 1 && c->head_stride < 0) || (c->page_size > 1 && c->token_stride < 0))
+        return refused(where, "strides must not be negative");
+    return BLK_OK;
+}
+
+bool rows_overlap(const blk_paged_cache_t* c) {
+    struct Dim { int64_t stride, size; } d[3] = {{c->page_stride, c->pages}, {c->head_stride, c->heads}, {c->token_stride, c->page_size}};
+    std::sort(d, d + 3, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+    int64_t span = c->head_dim;  // elements from the first to behind the last row of the dimensions so far
+    for (const Dim& x : d) {
+        if (x.size <= 1) continue;
+        if (x.stride < span) return true;
+        span += (x.size - 1) * x.stride;
+    }
+    return false;
+}
+
+int current_sms(const char* where, int* sms) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_fail(where, e);
+    }
+    return BLK_OK;
+}
+
+int check_paged_attention(const char* where, const blk_paged_cache_t* c, int64_t heads, int64_t requests, int64_t columns) {
+    const int rc = check_paged_cache(where, c);
+    if (rc != BLK_OK) return rc;
+    if (c->head_dim > 256) return refused(where, "head_dim must be at most 256", BLK_ERR_UNSUPPORTED);
+    if (heads < 1 || heads % c->heads || heads > 0xffffLL) return refused(where, "the query heads must be a multiple of the cache's, at most 65535");
+    if (requests < 0 || requests > 0x7fffffffLL || columns < 0 || columns > 0x7fffffffLL) return refused(where, "requests and columns must be 0 to 2^31 - 1");
+    return BLK_OK;
+}
+int64_t capacity_of(const blk_paged_cache_t* c, int64_t columns) { return std::min<int64_t>(columns * c->page_size, 0x7fffffffLL); }
+int64_t paged_workspace(const BlkPagedShape& s) { return (int64_t)s.blocks * (int64_t)sizeof(int4) + s.work_floats * (int64_t)sizeof(float); }
+
+}  // namespace
+
+extern "C" int blk_paged_slots(const int32_t* lengths, const int32_t* new_tokens, int64_t requests, int32_t* page_table,
+                               int64_t table_stride, int64_t columns, const int32_t* free_pages, int64_t num_free, const int32_t* taken,
+                               int64_t page_size, int64_t* slots, int64_t tokens, int32_t* lengths_out, int32_t* taken_out,
+                               void* cuda_stream) {
+    static const char where[] = "blk_paged_slots";
+    BlkRange range(where);
+    if (requests < 0 || requests > 0x7fffffffLL - 1024 || columns < 0 || columns > 0x7fffffffLL || num_free < 0 || tokens < 0)
+        return refused(where, "negative or too large extent");
+    if (page_size < 1 || page_size > (1LL << 30)) return refused(where, "the page size must be 1 to 2^30 tokens");
+    if (requests > 1 && table_stride < columns) return refused(where, "rows of the page table overlap");
+    if (!taken || !taken_out || (requests && (!lengths || !new_tokens || !lengths_out)) || (requests && columns && !page_table) ||
+        (num_free && !free_pages) || (tokens && !slots))
+        return refused(where, "null buffer");
+    BlkPagedSlotsParams p{};
+    p.lengths = lengths;
+    p.new_tokens = new_tokens;
+    p.table = page_table;
+    p.table_stride = table_stride;
+    p.free_pages = free_pages;
+    p.taken = taken;
+    p.slots = slots;
+    p.lengths_out = lengths_out;
+    p.taken_out = taken_out;
+    p.tokens = tokens;
+    p.num_free = num_free;
+    p.requests = (int)requests;
+    p.columns = (int)columns;
+    p.page = blk_divisor((uint32_t)page_size);
+    int sms = 0;
+    const int rc = current_sms(where, &sms);
+    if (rc != BLK_OK) return rc;
+    const cudaError_t e = blk_launch_paged_slots(p, sms, reinterpret_cast<cudaStream_t>(cuda_stream));
+    return e == cudaSuccess ? BLK_OK : cuda_fail(where, e);
+}
+
+extern "C" int blk_paged_append(const blk_paged_cache_t* c, const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                                int64_t v_row_stride, int64_t v_head_stride, const int64_t* slots, int64_t tokens, void* cuda_stream) {
+    static const char where[] = "blk_paged_append";
+    BlkRange range(where);
+    const int rc = check_paged_cache(where, c);
+    if (rc != BLK_OK) return rc;
+    if (rows_overlap(c)) return refused(where, "rows of the cache overlap");
+    if (tokens < 0 || tokens > 0x7fffffffLL) return refused(where, "tokens must be 0 to 2^31 - 1");
+    if (tokens == 0 || c->pages == 0) return BLK_OK;
+    if (!k || !v || !slots) return refused(where, "null buffer");
+    const int64_t e = bytes_of(c->dtype);
+    if (!aligned16(k) || !aligned16(v) || (tokens > 1 && (k_row_stride * e % 16 || v_row_stride * e % 16)) ||
+        (c->heads > 1 && (k_head_stride * e % 16 || v_head_stride * e % 16)))
+        return refused(where, "new rows must start on 16-byte boundaries", BLK_ERR_UNALIGNED);
+    BlkPagedAppendParams p{};
+    p.k = static_cast<const char*>(k);
+    p.v = static_cast<const char*>(v);
+    p.k_cache = static_cast<char*>(c->k);
+    p.v_cache = static_cast<char*>(c->v);
+    p.k_row_stride = k_row_stride * e;
+    p.k_head_stride = k_head_stride * e;
+    p.v_row_stride = v_row_stride * e;
+    p.v_head_stride = v_head_stride * e;
+    p.page_stride = c->page_stride * e;
+    p.head_stride = c->head_stride * e;
+    p.token_stride = c->token_stride * e;
+    p.slots = slots;
+    p.tokens = tokens;
+    p.num_slots = c->pages * c->page_size;
+    const int64_t chunks = c->head_dim * e / 16;
+    if (chunks * c->heads > 0x3fffffffLL) return refused(where, "heads x head_dim too large", BLK_ERR_UNSUPPORTED);
+    p.pieces = (int)(chunks * c->heads);
+    p.page = blk_divisor((uint32_t)c->page_size);
+    p.chunks = blk_divisor((uint32_t)chunks);
+    const cudaError_t err = blk_launch_paged_append(p, reinterpret_cast<cudaStream_t>(cuda_stream));
+    return err == cudaSuccess ? BLK_OK : cuda_fail(where, err);
+}
+
+extern "C" int blk_paged_attention_workspace(const blk_paged_cache_t* c, int64_t heads, int64_t requests, int64_t columns, int64_t* bytes) {
+    static const char where[] = "blk_paged_attention_workspace";
+    int rc = check_paged_attention(where, c, heads, requests, columns);
+    if (rc != BLK_OK) return rc;
+    if (!bytes) return refused(where, "null pointer");
+    int sms = 0;
+    rc = current_sms(where, &sms);
+    if (rc != BLK_OK) return rc;
+    *bytes = requests ? paged_workspace(blk_paged_shape(c->dtype, (int)c->head_dim, (int)(heads / c->heads), requests, c->heads,
+                                                        capacity_of(c, columns), sms))
+                      : 0;
+    return BLK_OK;
+}
+
+extern "C" int blk_paged_attention(const blk_paged_cache_t* c, const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t heads,
+                                   const int32_t* page_table, int64_t table_stride, int64_t columns, const int32_t* lengths,
+                                   int64_t requests, float scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                   void* cuda_stream) {
+    static const char where[] = "blk_paged_attention";
+    BlkRange range(where);
+    int rc = check_paged_attention(where, c, heads, requests, columns);
+    if (rc != BLK_OK) return rc;
+    if (requests == 0) return BLK_OK;
+    if (!q || !lengths || !out || !workspace || (columns && !page_table)) return refused(where, "null buffer");
+    if (requests > 1 && table_stride < 0) return refused(where, "strides must not be negative");
+    const int64_t e = bytes_of(c->dtype);
+    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (requests > 1 && q_row_stride * e % 16) || (heads > 1 && q_head_stride * e % 16))
+        return refused(where, "q, out and the workspace must be 16-byte aligned, rows of q on 16-byte boundaries", BLK_ERR_UNALIGNED);
+    int sms = 0;
+    rc = current_sms(where, &sms);
+    if (rc != BLK_OK) return rc;
+    BlkPagedAttnParams p{};
+    p.capacity = (int)capacity_of(c, columns);
+    p.group = (int)(heads / c->heads);
+    const BlkPagedShape s = blk_paged_shape(c->dtype, (int)c->head_dim, p.group, requests, c->heads, p.capacity, sms);
+    if (workspace_bytes < paged_workspace(s)) return refused(where, "the workspace is too small");
+    p.q = static_cast<const char*>(q);
+    p.k = static_cast<const char*>(c->k);
+    p.v = static_cast<const char*>(c->v);
+    p.q_row_stride = q_row_stride * e;
+    p.q_head_stride = q_head_stride * e;
+    p.page_stride = c->page_stride * e;
+    p.head_stride = c->head_stride * e;
+    p.token_stride = c->token_stride * e;
+    p.table = page_table;
+    p.table_stride = table_stride;
+    p.lengths = lengths;
+    p.requests = (int)requests;
+    p.q_units = s.q_units;
+    p.rows_unit = s.rows_unit;
+    p.units = (int)c->heads * s.q_units;
+    p.heads = (int)heads;
+    p.d = (int)c->head_dim;
+    p.pages = (int)c->pages;
+    p.page = blk_divisor((uint32_t)c->page_size);
+    p.out = out;
+    p.lse = lse;
+    p.parts = static_cast<int4*>(workspace);
+    p.work = reinterpret_cast<float*>(p.parts + s.blocks);
+    p.negate = scale < 0.f;
+    p.scale = p.negate ? -scale : scale;
+    if (p.scale == 0.f) p.scale = 1.17549435e-38f;  // softmax(0 * S) is the uniform distribution
+    p.c = p.scale * 1.4426950408889634f;
+    const cudaError_t err = blk_launch_paged_attn(p, s, c->dtype, reinterpret_cast<cudaStream_t>(cuda_stream));
+    return err == cudaSuccess ? BLK_OK : cuda_fail(where, err);
+}

@@ -258,3 +258,67 @@ cudaError_t blk_launch_attn_bwd_umma(const BlkFlashBwdParams& p, int keys, const
 cudaError_t blk_launch_attn_bwd_small(const BlkAttnBwdSmallParams& p, int D, int rows, int bf16, cudaStream_t st);
 cudaError_t blk_launch_scores_pipe(const BlkPackParams& p, int dtype_in, int sms, cudaStream_t st);
 cudaError_t blk_launch_softmax(const BlkSmxParams& p, int dtype, cudaStream_t st);
+
+// ---- paged cache (blk_paged.cu, blk_paged_attn.cu) ------------------------------------------------------
+// A number divided by the same one over and over: n / d = (mulhi(n, magic) + n) >> shift for n < 2^31, 1 <= d <= 2^30.
+struct BlkDivisor {
+    uint32_t d, magic, shift;
+};
+inline BlkDivisor blk_divisor(uint32_t d) {
+    uint32_t shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    return BlkDivisor{d, (uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
+}
+
+// Strides in bytes.
+struct BlkPagedAttnParams {
+    const char *q, *k, *v;
+    int64_t q_row_stride, q_head_stride, page_stride, head_stride, token_stride;
+    const int* table;
+    int64_t table_stride;  // entries
+    const int* lengths;
+    int capacity;          // tokens that a row of the table has pages for
+    int requests, units, q_units, rows_unit, group, heads, d, pages;
+    BlkDivisor page;
+    void* out;
+    float* lse;
+    float* work;
+    int4* parts;
+    float c, scale;        // |scale| log2(e), |scale|
+    int negate;            // scale < 0: the kernel takes -q
+};
+// How a call is cut: padded head dimension, units a key head's query rows are taken in, their rows and eights of rows,
+// blocks, and what these leave for the join.
+struct BlkPagedShape {
+    int DP, q_units, rows_unit, NT, blocks;
+    int64_t work_floats;
+};
+BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int64_t kv_heads, int64_t capacity, int sms);
+cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedShape& s, int dtype, cudaStream_t st);
+
+struct BlkPagedSlotsParams {
+    const int *lengths, *new_tokens;
+    int* table;
+    int64_t table_stride;
+    const int* free_pages;
+    const int* taken;
+    int64_t* slots;
+    int* lengths_out;
+    int* taken_out;
+    int64_t tokens, num_free;
+    int requests, columns;
+    BlkDivisor page;
+};
+cudaError_t blk_launch_paged_slots(const BlkPagedSlotsParams& p, int sms, cudaStream_t st);
+
+// Strides in bytes; chunks: 16-byte pieces of a row.
+struct BlkPagedAppendParams {
+    const char *k, *v;
+    char *k_cache, *v_cache;
+    int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride, page_stride, head_stride, token_stride;
+    const int64_t* slots;
+    int64_t tokens, num_slots;
+    int pieces;  // heads x chunks
+    BlkDivisor page, chunks;
+};
+cudaError_t blk_launch_paged_append(const BlkPagedAppendParams& p, cudaStream_t st);

@@ -1,0 +1,728 @@
+// Attention of one new token per request over its cached keys and values, held in pages.
+//
+//   s_j = scale q . k_j for the tokens j of a request,  m = max s_j,  l = sum exp(s_j - m),  out = sum exp(s_j - m) v_j / l
+//
+// All keys and values are read once and little is done with each, so the bytes bound it (2 x tokens x heads x d).  The work is one
+// list of tiles of 64 tokens, (request, key head, tile) in this order, which every block cuts into equal ranges by itself: it
+// adds up the lengths on the way in, so no length is ever read by the host.  A block's tiles arrive through a ring of
+// asynchronous 16-byte copies that runs on over the end of a request or head.  A warp owns 16 tokens of every tile and
+// the part of the ring they go through: within a head nothing but its own copies is waited for.  Where a head is done, the four
+// warps' maxima, sums and weighted values are put together; where it goes on in another block, they go to the workspace, and
+// a second kernel joins the parts of the heads that were cut (at most two parts a block, so the workspace does
+// not grow with the lengths).  No atomics: the same call gives the same bits.
+#include "blk_device.cuh"
+#include "blk_kernels.h"
+
+namespace {
+
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+    const int n = there ? 16 : 0;  // 0: sixteen zeros, nothing is read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float4 lds128(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+// Weight of a part whose maximum is m where the whole's is top.  -inf: the part saw nothing, or scores of -inf alone.
+__device__ __forceinline__ float part_weight(float m, float top, float c) {
+    if (m == -INFINITY) return top == -INFINITY ? 1.f : 0.f;
+    return blk_exp2((m - top) * c);
+}
+
+// ---- the arithmetic of one warp, 16-bit types ---------------------------------------------------------
+// Scores and values on the tensor cores with the tokens as the wide side: S^T = K Q^T is (16 tokens x 8 query rows), O^T = V^T P^T is
+// (d x 8 query rows), so the query heads that share a key head fill the narrow side and nothing is padded beyond eight.  P goes
+// from accumulator to operand by one 8 x 8 transposition in registers.  It enters as the sum of two 16-bit numbers: rounded once
+// it would add as much error as the rounding of the result does, and the second product costs no time next to the copies.
+// fp16 holds nothing below 2^-24: there P is 2^14 times as large, so that what it loses is below 2^-38 of the largest.
+// The first of the two is cut, not rounded, and the second never zero: both are positive, so that an infinite value stays one.
+template <typename Tag> struct PSplit;
+template <> struct PSplit<BlkBf16Tag> {
+    static constexpr float SCALE = 1.f;
+    static __device__ __forceinline__ uint32_t hi(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+    static __device__ __forceinline__ uint32_t lo(float a, float b, uint32_t h) {
+        return BlkCvt<BlkBf16Tag>::pack2(fmaxf(a - __uint_as_float(h << 16), 1.17549435e-38f), fmaxf(b - __uint_as_float(h & 0xffff0000u), 1.17549435e-38f));
+    }
+};
+template <> struct PSplit<BlkHalfTag> {
+    static constexpr float SCALE = 16384.f;
+    static __device__ __forceinline__ uint32_t hi(float a, float b) {
+        uint32_t h;
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;\n" : "=r"(h) : "f"(b), "f"(a));
+        return h;
+    }
+    static __device__ __forceinline__ uint32_t lo(float a, float b, uint32_t h) {
+        const float2 r = __half22float2(*reinterpret_cast<__half2*>(&h));
+        return BlkCvt<BlkHalfTag>::pack2(fmaxf(a - r.x, 5.9604645e-8f), fmaxf(b - r.y, 5.9604645e-8f));
+    }
+};
+
+template <typename Tag_, int DP_, int NT_, int STAGES_, int CTAS_>
+struct Math16 {
+    typedef Tag_ Tag;
+    static constexpr int DP = DP_, NT = NT_, GU = 8 * NT, E = 2, TW = 16, STAGES = STAGES_, CTAS = CTAS_, RB = DP * E, EXTRA = 0;
+    uint32_t qf[DP / 16][NT][2];
+    float o[DP / 16][NT][4];
+    float m[NT][2], l[NT][2];
+    bool seen;
+
+    __device__ __forceinline__ void begin(const BlkPagedAttnParams& p, const char* q, int rows, uint32_t, int lane) {
+        const uint32_t flip = p.negate ? 0x80008000u : 0u;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = n * 8 + lane / 4;
+            const char* at = q + row * p.q_head_stride + (lane & 3) * 4;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int col = kk * 16 + h * 8;
+                    qf[kk][n][h] = row < rows && col < p.d ? *reinterpret_cast<const uint32_t*>(at + col * 2) ^ flip : 0u;
+                }
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int mm = 0; mm < DP / 16; ++mm)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mm][n][e] = 0.f;
+        }
+        seen = false;
+    }
+
+    __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float c, uint32_t, int lane) {
+        seen = true;
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+        {
+            const int row = lane & 15;
+            const uint32_t base = sK + row * RB, x = ((lane >> 4) ^ (row & 7)) << 4;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                uint32_t a[4];
+                blk_ldmatrix_x4(a, base + ((kk * 32) ^ x));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) blk_mma16816<Tag>(s[n], a[0], a[1], a[2], a[3], qf[kk][n][0], qf[kk][n][1]);
+            }
+        }
+        const bool v0 = mask >> (lane / 4) & 1, v1 = mask >> (lane / 4 + 8) & 1;
+        uint32_t hi[NT][2], lo[NT][2];
+        float alpha[NT][2];
+        bool grew = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float t = fmaxf(v0 ? s[n][e] : -INFINITY, v1 ? s[n][2 + e] : -INFINITY);
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                const float top = fmaxf(m[n][e], t), ref = top == -INFINITY ? 0.f : top;
+                alpha[n][e] = blk_exp2((m[n][e] - ref) * c);
+                grew |= top > m[n][e];
+                m[n][e] = top;
+                s[n][e] = v0 ? blk_exp2((s[n][e] - ref) * c) : 0.f;
+                s[n][2 + e] = v1 ? blk_exp2((s[n][2 + e] - ref) * c) : 0.f;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float a = s[n][2 * h] * PSplit<Tag>::SCALE, b = s[n][2 * h + 1] * PSplit<Tag>::SCALE;
+                const uint32_t w = PSplit<Tag>::hi(a, b);
+                hi[n][h] = movmatrix(w);
+                lo[n][h] = movmatrix(PSplit<Tag>::lo(a, b, w));
+            }
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                l[n][0] *= alpha[n][0];
+                l[n][1] *= alpha[n][1];
+#pragma unroll
+                for (int mm = 0; mm < DP / 16; ++mm)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[mm][n][e] *= alpha[n][e & 1];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) l[n][e] += s[n][e] + s[n][2 + e];
+        {
+            const int row = (lane & 7) + ((lane >> 4) << 3);
+            const uint32_t base = sV + row * RB, x = (((lane >> 3) & 1) ^ (row & 7)) << 4;
+#pragma unroll
+            for (int mm = 0; mm < DP / 16; ++mm) {
+                uint32_t a[4];
+                blk_ldmatrix_x4_trans(a, base + ((mm * 32) ^ x));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    blk_mma16816<Tag>(o[mm][n], a[0], a[1], a[2], a[3], hi[n][0], hi[n][1]);
+                    blk_mma16816<Tag>(o[mm][n], a[0], a[1], a[2], a[3], lo[n][0], lo[n][1]);
+                }
+            }
+        }
+    }
+
+    // this warp's maxima and sums, a float for each query row
+    __device__ __forceinline__ void stats(float* sm, float* sl, int lane) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float t = l[n][e];
+                t += __shfl_xor_sync(0xffffffffu, t, 4);
+                t += __shfl_xor_sync(0xffffffffu, t, 8);
+                t += __shfl_xor_sync(0xffffffffu, t, 16);
+                if (lane < 4) {
+                    sm[n * 8 + lane * 2 + e] = m[n][e];
+                    sl[n * 8 + lane * 2 + e] = seen && m[n][e] == -INFINITY ? NAN : t;  // scores of -inf alone: 0 / 0
+                }
+            }
+    }
+    // this warp's weighted values of query rows 8n .. 8n+7, rows of DP + 4 floats; w: the rows' weights
+    __device__ __forceinline__ void put(int n_, float* dst, const float* w, int lane) {
+        const int q = (lane & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            if (n == n_) {
+                const float w0 = w[n * 8 + q] * (1.f / PSplit<Tag>::SCALE), w1 = w[n * 8 + q + 1] * (1.f / PSplit<Tag>::SCALE);
+#pragma unroll
+                for (int mm = 0; mm < DP / 16; ++mm) {
+                    float* at = dst + q * (DP + 4) + mm * 16 + lane / 4;
+                    at[0] = o[mm][n][0] * w0;
+                    at[DP + 4] = o[mm][n][1] * w1;
+                    at[8] = o[mm][n][2] * w0;
+                    at[DP + 4 + 8] = o[mm][n][3] * w1;
+                }
+            }
+    }
+};
+
+// ---- the same in 32 bits -------------------------------------------------------------------------------
+// A lane holds one token (part of its row: 32 / TW lanes share one) for the scores and DP / 32 columns for the values; q and the
+// weights are broadcast from shared memory.
+struct BlkFloatTag {};
+template <int DP_, int TW_, int STAGES_, int CTAS_>
+struct Math32 {
+    typedef BlkFloatTag Tag;
+    static constexpr int DP = DP_, NT = 1, GU = 8, E = 4, TW = TW_, STAGES = STAGES_, CTAS = CTAS_, RB = DP * E, PARTS = 32 / TW, W = DP / 32;
+    static constexpr int EXTRA = 8 * DP * 4 + WARPS * TW * 8 * 4;  // q, weights of every warp
+    float o[8][W];
+    float m[8], l[8];
+    bool seen;
+
+    __device__ __forceinline__ void begin(const BlkPagedAttnParams& p, const char* q, int rows, uint32_t sx, int) {
+        for (int i = threadIdx.x; i < 8 * DP; i += THREADS) {
+            const int row = i / DP, col = i % DP;
+            float v = row < rows && col < p.d ? reinterpret_cast<const float*>(q + row * p.q_head_stride)[col] : 0.f;
+            blk_sts_f32(sx + i * 4, p.negate ? -v : v);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+#pragma unroll
+            for (int j = 0; j < W; ++j) o[i][j] = 0.f;
+        }
+        seen = false;
+    }
+
+    __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float c, uint32_t sx, int lane) {
+        seen = true;
+        const int tok = lane % TW, part = lane / TW;
+        const bool valid = mask >> tok & 1;
+        float s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = 0.f;
+#pragma unroll 4
+        for (int j = 0; j < DP / 4 / PARTS; ++j) {
+            const int ch = j * PARTS + part;
+            const float4 k = lds128(sK + tok * RB + ((ch ^ (tok & 7)) << 4));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 q = lds128(sx + (i * DP + ch * 4) * 4);
+                s[i] = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, s[i]))));
+            }
+        }
+        const uint32_t sp = sx + 8 * DP * 4 + (threadIdx.x / 32) * (TW * 8 * 4);
+        __syncwarp();  // (the weights of the tile before are read)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int x = TW; x < 32; x *= 2) s[i] += __shfl_xor_sync(0xffffffffu, s[i], x);
+            float t = valid ? s[i] : -INFINITY;
+#pragma unroll
+            for (int x = 1; x < TW; x *= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+            const float top = fmaxf(m[i], t), ref = top == -INFINITY ? 0.f : top;
+            if (top > m[i]) {  // (the same for the whole warp)
+                const float alpha = blk_exp2((m[i] - ref) * c);
+                l[i] *= alpha;
+#pragma unroll
+                for (int j = 0; j < W; ++j) o[i][j] *= alpha;
+            }
+            m[i] = top;
+            s[i] = valid ? blk_exp2((s[i] - ref) * c) : 0.f;
+            if (part == 0) {
+                l[i] += s[i];
+                blk_sts_f32(sp + (tok * 8 + i) * 4, s[i]);
+            }
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int t = 0; t < TW; ++t) {
+            const float4 a = lds128(sp + t * 32), b = lds128(sp + t * 32 + 16);
+            const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            float v[W];
+            if (W == 2) {
+                const uint32_t at = sV + t * RB + (((lane >> 1) ^ (t & 7)) << 4) + (lane & 1) * 8;
+                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];\n" : "=f"(v[0]), "=f"(v[1]) : "r"(at));
+            } else {
+#pragma unroll
+                for (int j = 0; j < W / 4; ++j) {
+                    const float4 x = lds128(sV + t * RB + (((lane + 32 * j) ^ (t & 7)) << 4));
+                    v[(4 * j) % W] = x.x;
+                    v[(4 * j + 1) % W] = x.y;
+                    v[(4 * j + 2) % W] = x.z;
+                    v[(4 * j + 3) % W] = x.w;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j) o[i][j] = fmaf(w[i], v[j], o[i][j]);
+        }
+    }
+
+    __device__ __forceinline__ void stats(float* sm, float* sl, int lane) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float t = l[i];
+#pragma unroll
+            for (int x = 1; x < TW; x *= 2) t += __shfl_xor_sync(0xffffffffu, t, x);
+            if (lane == 0) {
+                sm[i] = m[i];
+                sl[i] = seen && m[i] == -INFINITY ? NAN : t;
+            }
+        }
+    }
+    __device__ __forceinline__ void put(int, float* dst, const float* w, int lane) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = w[i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const int col = W == 2 ? lane * 2 + j : (j / 4) * 128 + lane * 4 + (j & 3);
+                dst[i * (DP + 4) + col] = o[i][j] * x;
+            }
+        }
+    }
+};
+
+// ---- shared memory -------------------------------------------------------------------------------------
+template <typename M>
+struct Lay {
+    static constexpr int TILE = WARPS * M::TW;
+    static constexpr int HALF = M::TW * M::RB;                       // a warp's keys, or values, of a stage
+    static constexpr int RING = WARPS * M::STAGES * 2 * HALF;
+    static constexpr int MERGE = WARPS * 8 * (M::DP + 4) * 4;
+    static constexpr int STATS = (3 * WARPS + 2) * M::GU * 4;        // maxima, sums, weights of the warps; those of the block
+    static constexpr int MASKS = WARPS * M::STAGES * 4;
+    static constexpr int SCHED = 64;
+    static constexpr int BYTES = RING + MERGE + M::EXTRA + STATS + MASKS + SCHED;
+};
+
+// Where a block is in the list of tiles: tile t of n of unit u (a key head, or a part of its query rows) of request r.
+struct Walk {
+    int r, u, t, n, len, ahead;
+};
+__device__ __forceinline__ int held(const BlkPagedAttnParams& p, int r) {
+    return min(max(p.lengths[r], 0), p.capacity);
+}
+template <int TILE>
+__device__ __forceinline__ int tiles_of(int len) { return max(1, (int)(((unsigned)len + TILE - 1) / TILE)); }  // (an empty request's result is written, too)
+template <int TILE>
+__device__ __forceinline__ void step(Walk& w, const BlkPagedAttnParams& p) {
+    if (++w.t < w.n) return;
+    w.t = 0;
+    if (++w.u < p.units) return;
+    w.u = 0;
+    ++w.r;
+    w.len = w.ahead;
+    w.n = tiles_of<TILE>(w.len);
+    w.ahead = w.r + 1 < p.requests ? held(p, w.r + 1) : 0;
+}
+
+template <typename Tag> struct Out;
+template <> struct Out<BlkHalfTag> {
+    static __device__ __forceinline__ void put4(void* out, int64_t at, float4 v) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(BlkCvt<BlkHalfTag>::pack2(v.x, v.y), BlkCvt<BlkHalfTag>::pack2(v.z, v.w));
+    }
+};
+template <> struct Out<BlkBf16Tag> {
+    static __device__ __forceinline__ void put4(void* out, int64_t at, float4 v) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(BlkCvt<BlkBf16Tag>::pack2(v.x, v.y), BlkCvt<BlkBf16Tag>::pack2(v.z, v.w));
+    }
+};
+template <> struct Out<BlkFloatTag> {
+    static __device__ __forceinline__ void put4(void* out, int64_t at, float4 v) { *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v; }
+};
+
+// Result of a head's row from its sum and weighted values.  No token at all: l = 0 and zeros.
+__device__ __forceinline__ float4 divided(float4 v, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    return make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+}
+__device__ __forceinline__ float row_log(float m, float l, float scale) { return l == 0.f ? -INFINITY : m * scale + logf(l); }
+
+template <typename M>
+__global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const BlkPagedAttnParams p) {
+    typedef Lay<M> L;
+    constexpr int DP = M::DP, GU = M::GU, TW = M::TW, RB = M::RB, STAGES = M::STAGES, TILE = L::TILE, CPR = RB / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* const merge = reinterpret_cast<float*>(smem + L::RING);
+    float* const sm_m = reinterpret_cast<float*>(smem + L::RING + L::MERGE + M::EXTRA);
+    float* const sm_l = sm_m + WARPS * GU;
+    float* const sm_w = sm_l + WARPS * GU;
+    float* const top_m = sm_w + WARPS * GU;
+    float* const top_l = top_m + GU;
+    uint32_t* const masks = reinterpret_cast<uint32_t*>(top_l + GU) + threadIdx.x / 32 * STAGES;
+    int64_t* const sched = reinterpret_cast<int64_t*>(smem + L::RING + L::MERGE + M::EXTRA + L::STATS + L::MASKS);
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const uint32_t ring = blk_smem_u32(smem) + warp * (STAGES * 2 * L::HALF), extra = blk_smem_u32(smem) + L::RING + L::MERGE;
+    const int chunks = p.d * M::E / 16;
+    if (chunks < CPR) {  // columns beyond d take part in the products, and no copy writes them
+        for (int i = lane; i < STAGES * 2 * L::HALF / 16; i += 32)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(ring + i * 16), "r"(0) : "memory");
+        __syncwarp();
+    }
+    blk_grid_wait();
+
+    // The lengths, added up: a run of requests for every thread.
+    Walk cw;
+    int64_t lo, hi;
+    {
+        const int per = (p.requests + THREADS - 1) / THREADS, r0 = min(tid * per, p.requests), r1 = min(r0 + per, p.requests);
+        int64_t mine = 0;
+        for (int r = r0; r < r1; ++r) mine += tiles_of<TILE>(held(p, r));
+        int64_t before = mine;
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, before, x);
+            if (lane >= x) before += y;
+        }
+        if (lane == 31) sched[warp] = before;
+        __syncthreads();
+        int64_t all = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) before += sched[w];
+            all += sched[w];
+        }
+        before -= mine;
+        all *= p.units;
+        const int64_t blocks = min((int64_t)gridDim.x, all);
+        if (blockIdx.x >= blocks) {
+            if (tid == 0) p.parts[blockIdx.x] = make_int4(0, 0, 0, 0);
+            return;
+        }
+        lo = blockIdx.x * all / blocks;
+        hi = (blockIdx.x + 1) * all / blocks;
+        const int64_t x = lo / p.units;
+        if (x >= before && x < before + mine) {
+            int r = r0;
+            int64_t at = before;
+            int n = tiles_of<TILE>(held(p, r));
+            while (x >= at + n) {
+                at += n;
+                n = tiles_of<TILE>(held(p, ++r));
+            }
+            sched[4] = r;
+            sched[5] = lo - at * p.units;
+        }
+        if (tid == 0) {
+            sched[6] = all;
+            sched[7] = blocks;
+        }
+        __syncthreads();
+        cw.r = (int)sched[4];
+        cw.len = held(p, cw.r);
+        cw.n = tiles_of<TILE>(cw.len);
+        cw.u = (int)(sched[5] / cw.n);
+        cw.t = (int)(sched[5] % cw.n);
+        cw.ahead = cw.r + 1 < p.requests ? held(p, cw.r + 1) : 0;
+    }
+    const int64_t count = hi - lo;
+
+    // Copies.  A lane looks up the page of one of the warp's tokens, a tile before its rows are asked for.
+    Walk pw = cw;
+    int entry = -1;
+    int64_t inner = 0;
+    auto look = [&]() {
+        const unsigned tok = (unsigned)pw.t * TILE + warp * TW + lane;
+        entry = -1;
+        if (lane < TW && tok < (unsigned)pw.len) {
+            const unsigned col = (__umulhi(tok, p.page.magic) + tok) >> p.page.shift;
+            entry = p.table[pw.r * p.table_stride + col];
+            inner = (int64_t)(tok - col * p.page.d) * p.token_stride + (int64_t)(pw.u / p.q_units) * p.head_stride;
+        }
+    };
+    auto load = [&](int stage) {
+        const bool there = entry >= 0 && entry < p.pages;
+        const int64_t off = there ? entry * p.page_stride + inner : -1;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) masks[stage] = mask;
+        if (mask) {
+            const uint32_t sK = ring + stage * (2 * L::HALF), sV = sK + L::HALF;
+#pragma unroll
+            for (int i = 0; i < TW * CPR / 32; ++i) {
+                const int idx = i * 32 + lane, row = idx / CPR, ch = idx % CPR;
+                const int64_t o = __shfl_sync(0xffffffffu, off, row);
+                if (ch < chunks) {
+                    const int64_t at = (o < 0 ? 0 : o) + ch * 16;
+                    const uint32_t dst = row * RB + ((ch ^ (row & 7)) << 4);
+                    if (o >= 0) cp_async16(sK + dst, p.k + at, true);
+                    cp_async16(sV + dst, p.v + at, o >= 0);
+                }
+            }
+        }
+    };
+    look();
+    int64_t loaded = 0;
+    int into = 0;
+    auto next = [&]() {
+        if (loaded < count) {
+            load(into);
+            into = into + 1 == STAGES ? 0 : into + 1;
+            if (++loaded < count) {
+                step<TILE>(pw, p);
+                look();
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll 1
+    for (int s = 0; s < STAGES - 1; ++s) next();
+
+    M math;
+    int stage = 0, part_of = 0;
+    int4 part = make_int4(0, 0, 0, 0);
+    for (int64_t i = 0; i < count; ++i) {
+        const int kv = cw.u / p.q_units, first = (cw.u % p.q_units) * p.rows_unit, rows = min(p.rows_unit, p.group - first);
+        const int64_t head0 = (int64_t)kv * p.group + first;
+        if (i == 0 || cw.t == 0) math.begin(p, p.q + cw.r * p.q_row_stride + head0 * p.q_head_stride, rows, extra, lane);
+        cp_wait<STAGES - 2>();
+        __syncwarp();
+        next();
+        const uint32_t mask = masks[stage];
+        if (mask) {
+            const uint32_t sK = ring + stage * (2 * L::HALF);
+            math.tile(sK, sK + L::HALF, mask, p.c, extra, lane);
+        }
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        const bool ends = cw.t + 1 == cw.n;
+        if (ends || i + 1 == count) {
+            const bool begins = i >= cw.t;
+            math.stats(sm_m + warp * GU, sm_l + warp * GU, lane);
+            __syncthreads();
+            if (tid < GU) {
+                float top = sm_m[tid], sum = 0.f;
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w * GU + tid]);
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    const float x = part_weight(sm_m[w * GU + tid], top, p.c);
+                    sm_w[w * GU + tid] = x;
+                    if (x != 0.f) sum += x * sm_l[w * GU + tid];
+                }
+                top_m[tid] = top;
+                top_l[tid] = sum;
+            }
+            __syncthreads();
+            const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
+            float* const ws = p.work + (int64_t)slot * (GU * DP + 2 * GU);
+#pragma unroll 1
+            for (int n = 0; n < M::NT; ++n) {
+                math.put(n, merge + warp * (8 * (DP + 4)), sm_w + warp * GU, lane);
+                __syncthreads();
+                for (int x = tid; x < 8 * DP / 4; x += THREADS) {
+                    const int q = x / (DP / 4), col = x % (DP / 4) * 4, row = n * 8 + q;
+                    if (row >= rows || col >= p.d) continue;
+                    float4 v = *reinterpret_cast<const float4*>(merge + q * (DP + 4) + col);
+#pragma unroll
+                    for (int w = 1; w < WARPS; ++w) {
+                        const float4 y = *reinterpret_cast<const float4*>(merge + (w * 8 + q) * (DP + 4) + col);
+                        v.x += y.x;
+                        v.y += y.y;
+                        v.z += y.z;
+                        v.w += y.w;
+                    }
+                    if (begins && ends) {
+                        const int64_t head = (int64_t)cw.r * p.heads + head0 + row;
+                        Out<typename M::Tag>::put4(p.out, head * p.d + col, divided(v, top_l[row]));
+                        if (p.lse && col == 0) p.lse[head] = row_log(top_m[row], top_l[row], p.scale);
+                    } else {
+                        *reinterpret_cast<float4*>(ws + row * DP + col) = v;
+                        if (col == 0) {
+                            ws[GU * DP + row] = top_m[row];
+                            ws[GU * DP + GU + row] = top_l[row];
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+            if (begins && !ends) {  // the head goes on in the blocks up to the one that has its last tile
+                const int64_t last = lo + i - cw.t + cw.n - 1;
+                part_of = (int)(((last + 1) * sched[7] - 1) / sched[6]) - (int)blockIdx.x + 1;
+                part = make_int4(part_of, cw.r, cw.u, 0);
+            }
+        }
+        if (i + 1 < count) step<TILE>(cw, p);
+    }
+    cp_wait<0>();
+    if (tid == 0) p.parts[blockIdx.x] = part;
+}
+
+// Joins the parts of the heads that were cut: block (c, y) those of the head that begins in block c and goes on, four query rows
+// each, four warps to a row.
+template <typename Tag, int DP>
+__global__ void __launch_bounds__(512) blk_paged_join_kernel(const BlkPagedAttnParams p, int GU) {
+    __shared__ float sums[16][DP];
+    __shared__ float denom[16];
+    blk_grid_wait();
+    const int4 part = p.parts[blockIdx.x];
+    const int n = part.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, sub = warp / 4, row = blockIdx.y * 4 + warp % 4;
+    if (n == 0) return;
+    const int kv = part.z / p.q_units, first = (part.z % p.q_units) * p.rows_unit, rows = min(p.rows_unit, p.group - first);
+    if ((int)blockIdx.y * 4 >= rows) return;
+    const bool mine = row < rows;
+    const int64_t size = GU * DP + 2 * GU;
+    const float* const base = p.work + 2 * (int64_t)blockIdx.x * size;  // part i > 0 is the first of block c + i
+    auto at = [&](int i) { return base + (2 * (int64_t)i + (i == 0)) * size; };
+    float top = -INFINITY;
+    if (mine)
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, at(i)[GU * DP + row]);
+#pragma unroll
+    for (int x = 1; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    float acc[DP / 32], sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) acc[j] = 0.f;
+    if (mine) {
+#pragma unroll 4
+        for (int i = sub; i < n; i += 4) {
+            const float* a = at(i);
+            const float w = part_weight(a[GU * DP + row], top, p.c);
+            const float l = a[GU * DP + GU + row];
+            if (w != 0.f) sum += w * l;
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j)
+                if (lane + 32 * j < p.d) acc[j] = fmaf(w, a[row * DP + lane + 32 * j], acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) sums[warp][lane + 32 * j] = acc[j];
+    if (lane == 0) denom[warp] = sum;
+    __syncthreads();
+    const int r = warp % 4, col = lane * 4 + (warp / 4) * 128;  // (the first eight warps: 256 columns of a row)
+    if (!mine || col >= p.d || col >= DP) return;
+    const float l = denom[r] + denom[4 + r] + denom[8 + r] + denom[12 + r];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const float4 y = *reinterpret_cast<const float4*>(&sums[4 * s + r][col]);
+        v.x += y.x;
+        v.y += y.y;
+        v.z += y.z;
+        v.w += y.w;
+    }
+    const int64_t head = (int64_t)part.y * p.heads + (int64_t)kv * p.group + first + row;
+    Out<Tag>::put4(p.out, head * p.d + col, divided(v, l));
+    if (p.lse && col == 0) p.lse[head] = row_log(top, l, p.scale);
+}
+
+// The kernels: padded head dimension, query rows of a unit in eights, stages, blocks on an SM.
+template <typename Tag> struct Kernels16 {
+    typedef Math16<Tag, 64, 1, 4, 3> D64N1;
+    typedef Math16<Tag, 64, 2, 4, 3> D64N2;
+    typedef Math16<Tag, 64, 3, 4, 2> D64N3;
+    typedef Math16<Tag, 64, 4, 4, 2> D64N4;
+    typedef Math16<Tag, 128, 1, 3, 2> D128N1;
+    typedef Math16<Tag, 128, 2, 3, 2> D128N2;
+    typedef Math16<Tag, 256, 1, 3, 1> D256N1;
+};
+typedef Math32<64, 16, 3, 2> F64;
+typedef Math32<128, 16, 3, 1> F128;
+typedef Math32<256, 8, 2, 1> F256;
+
+// f(the kernel's type) for what a call needs
+template <typename M> struct Of { typedef M T; };
+template <typename F>
+auto with_kernel(int dtype, int DP, int NT, F f) {
+    auto half = [&](auto tag) {
+        typedef Kernels16<decltype(tag)> K;
+        if (DP == 64) {
+            if (NT == 1) return f(Of<typename K::D64N1>{});
+            if (NT == 2) return f(Of<typename K::D64N2>{});
+            if (NT == 3) return f(Of<typename K::D64N3>{});
+            return f(Of<typename K::D64N4>{});
+        }
+        if (DP == 128) return NT == 1 ? f(Of<typename K::D128N1>{}) : f(Of<typename K::D128N2>{});
+        return f(Of<typename K::D256N1>{});
+    };
+    if (dtype == BLK_F16) return half(BlkHalfTag{});
+    if (dtype == BLK_BF16) return half(BlkBf16Tag{});
+    return DP == 64 ? f(Of<F64>{}) : DP == 128 ? f(Of<F128>{}) : f(Of<F256>{});
+}
+
+}  // namespace
+
+// Query rows that share a key head are taken together as far as registers hold their results; more of them are units of their
+// own, which read the keys again.
+BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int64_t kv_heads, int64_t capacity, int sms) {
+    BlkPagedShape s{};
+    s.DP = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+    const int most = dtype == BLK_F32 ? 8 : s.DP == 64 ? 32 : s.DP == 128 ? 16 : 8;
+    s.q_units = (group + most - 1) / most;
+    s.rows_unit = (group + s.q_units - 1) / s.q_units;
+    s.NT = (s.rows_unit + 7) / 8;
+    int tile = 0, ctas = 0;
+    with_kernel(dtype, s.DP, s.NT, [&](auto m) {
+        typedef typename decltype(m)::T M;
+        tile = Lay<M>::TILE;
+        ctas = M::CTAS;
+    });
+    const int64_t tiles = capacity > 0 ? (capacity + tile - 1) / tile : 1, room = (int64_t)ctas * sms;
+    const int64_t units = requests * kv_heads * s.q_units;
+    s.blocks = (int)(units >= room || tiles >= room || units * tiles >= room ? room : units * tiles);
+    s.work_floats = (int64_t)s.blocks * 2 * (8 * s.NT) * (s.DP + 2);
+    return s;
+}
+
+cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedShape& s, int dtype, cudaStream_t st) {
+    const int GU = 8 * s.NT;
+    return with_kernel(dtype, s.DP, s.NT, [&](auto m) {
+        typedef typename decltype(m)::T M;
+        auto kern = blk_paged_attn_kernel<M>;
+        cudaError_t e = blk_func_smem(reinterpret_cast<const void*>(kern), Lay<M>::BYTES);
+        if (e != cudaSuccess) return e;
+        e = blk_launch(true, kern, dim3((unsigned)s.blocks), dim3(THREADS), (size_t)Lay<M>::BYTES, st, p);
+        if (e != cudaSuccess || s.blocks == 1) return e;
+        return blk_launch(true, blk_paged_join_kernel<typename M::Tag, M::DP>, dim3((unsigned)s.blocks, (unsigned)(s.rows_unit + 3) / 4), dim3(512),
+                          (size_t)0, st, p, GU);
+    });
+}

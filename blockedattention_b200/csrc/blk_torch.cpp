@@ -883,7 +883,152 @@ Tensor py_scores_token_major(PyObject* const* a) {
     return out;
 }
 
+// ---- the paged cache -----------------------------------------------------------------------------------
+// No plans and no lists here: lengths, tables and slots stay on the GPU, and the kernels cut the work up by themselves.
+const Tensor& cuda_tensor(const char* name, PyObject* o) {
+    TORCH_CHECK(THPVariable_Check(o), name, " must be CUDA Tensor");
+    const Tensor& t = THPVariable_Unpack(o);
+    TORCH_CHECK(t.is_cuda(), name, " must be CUDA Tensor");
+    return t;
+}
+const Tensor& index_tensor(const char* name, PyObject* o, int64_t dim, at::ScalarType type, c10::Device dev) {
+    const Tensor& t = cuda_tensor(name, o);
+    TORCH_CHECK(t.scalar_type() == type && t.dim() == dim && t.device() == dev, name, " must be a tensor of ", type, " with ", dim,
+                " dimension(s) on ", dev);
+    TORCH_CHECK(dim == 2 ? t.numel() == 0 || t.size(1) == 1 || t.stride(1) == 1 : t.is_contiguous(), name, " must be contiguous", dim == 2 ? " along its rows" : "");
+    return t;
+}
+int64_t as_int(const char* name, PyObject* o) {
+    const int64_t v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK(v >= 0, name, " must not be negative");
+    return v;
+}
+// What a kernel writes to in place: its version moves on, which is what tells a list of that tensor that was remembered, or a
+// graph that has saved it.
+void written(const char* name, const Tensor& t) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name, " is written in place and must not require a gradient");
+    torch::autograd::impl::bump_version(t);
+}
+
+blk_paged_cache_t cache_of(const Tensor& k, const Tensor& v) {
+    TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == v.device(),
+                "kCache and vCache must both have shape (pages, heads, pageSize, d), one type and one device");
+    TORCH_CHECK(k.size(3) <= 1 || (k.stride(3) == 1 && v.stride(3) == 1), "kCache and vCache must be contiguous along d");
+    for (int i = 0; i < 3; ++i)
+        TORCH_CHECK(k.size(i) <= 1 || k.stride(i) == v.stride(i), "kCache and vCache must have the same strides");
+    blk_paged_cache_t c{};
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.pages = k.size(0);
+    c.heads = k.size(1);
+    c.page_size = k.size(2);
+    c.head_dim = k.size(3);
+    c.page_stride = k.stride(0);
+    c.head_stride = k.stride(1);
+    c.token_stride = k.stride(2);
+    c.dtype = dtype_code(k.scalar_type());
+    return c;
+}
+
+// paged_slots(lengths, newTokens, pageTable, freePages, taken, pageSize, tokens, advance) -> (slots, lengths, taken)
+PyObject* py_paged_slots(PyObject* const* a) {
+    const c10::Device dev = cuda_tensor("lengths", a[0]).device();
+    const Tensor &lengths = index_tensor("lengths", a[0], 1, at::kInt, dev), &added = index_tensor("newTokens", a[1], 1, at::kInt, dev),
+                 &table = index_tensor("pageTable", a[2], 2, at::kInt, dev), &pages = index_tensor("freePages", a[3], 1, at::kInt, dev),
+                 &taken = index_tensor("taken", a[4], 1, at::kInt, dev);
+    const int64_t size = as_int("pageSize", a[5]), tokens = as_int("tokens", a[6]), B = lengths.numel();
+    const bool advance = as_bool(a[7]);
+    TORCH_CHECK(added.numel() == B && table.size(0) == B, "lengths, newTokens and pageTable must have one entry or row for each request");
+    TORCH_CHECK(taken.numel() == 1, "taken must have one element");
+    Tensor slots, next, used;
+    {
+        const NoGil free;
+        c10::cuda::CUDAGuard guard(dev);
+        slots = at::detail::empty_cuda(at::IntArrayRef(&tokens, 1), at::kLong, dev, std::nullopt);
+        const int64_t one = 1;
+        next = advance ? lengths : Tensor(at::detail::empty_cuda(at::IntArrayRef(&B, 1), at::kInt, dev, std::nullopt));
+        used = advance ? taken : Tensor(at::detail::empty_cuda(at::IntArrayRef(&one, 1), at::kInt, dev, std::nullopt));
+        written("pageTable", table);
+        if (advance) {
+            written("lengths", lengths);
+            written("taken", taken);
+        }
+        auto ints = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+        ok(blk_paged_slots(ints(lengths), ints(added), B, ints(table), table.stride(0), table.size(1), ints(pages), pages.numel(), ints(taken),
+                           size, static_cast<int64_t*>(slots.data_ptr()), tokens, ints(next), ints(used), stream_of(dev)));
+    }
+    PyRef x(THPVariable_Wrap(slots)), y(THPVariable_Wrap(next)), z(THPVariable_Wrap(used));
+    return x.o && y.o && z.o ? PyTuple_Pack(3, x.o, y.o, z.o) : nullptr;
+}
+
+// paged_append(k, v, kCache, vCache, slots)
+PyObject* py_paged_append(PyObject* const* a) {
+    const Tensor &k = cuda_tensor("k", a[0]), &v = cuda_tensor("v", a[1]), &kc = cuda_tensor("kCache", a[2]), &vc = cuda_tensor("vCache", a[3]);
+    const c10::Device dev = kc.device();
+    const Tensor& slots = index_tensor("slots", a[4], 1, at::kLong, dev);
+    const blk_paged_cache_t c = cache_of(kc, vc);
+    TORCH_CHECK(k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) == c.heads && k.size(2) == c.head_dim && k.size(0) == slots.numel(),
+                "k and v must both have shape (tokens, heads, d) of the slots and the cache");
+    TORCH_CHECK(k.scalar_type() == kc.scalar_type() && v.scalar_type() == kc.scalar_type() && k.device() == dev && v.device() == dev,
+                "k and v must have the cache's type and device");
+    TORCH_CHECK(c.head_dim <= 1 || (k.stride(2) == 1 && v.stride(2) == 1), "k and v must be contiguous along d");
+    {
+        const NoGil free;
+        c10::cuda::CUDAGuard guard(dev);
+        written("kCache", kc);
+        written("vCache", vc);
+        ok(blk_paged_append(&c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                            static_cast<const int64_t*>(slots.data_ptr()), slots.numel(), stream_of(dev)));
+    }
+    Py_RETURN_NONE;
+}
+
+Tensor paged_attention(PyObject* const* a, Tensor* lse) {
+    const Tensor &q = cuda_tensor("q", a[0]), &kc = cuda_tensor("kCache", a[1]), &vc = cuda_tensor("vCache", a[2]);
+    const c10::Device dev = q.device();
+    const Tensor &table = index_tensor("pageTable", a[3], 2, at::kInt, dev), &lengths = index_tensor("lengths", a[4], 1, at::kInt, dev);
+    const double scale = as_double(a[5]);
+    const blk_paged_cache_t c = cache_of(kc, vc);
+    TORCH_CHECK(kc.scalar_type() == q.scalar_type() && kc.device() == dev, "q must have the cache's type and device");
+    TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim && (c.head_dim <= 1 || q.stride(2) == 1), "q must have shape (requests, heads, d), d that of the cache, contiguous along d");
+    const int64_t B = q.size(0), H = q.size(1);
+    TORCH_CHECK(lengths.numel() == B && table.size(0) == B, "lengths and pageTable must have one entry or row for each request");
+    const NoGil free;
+    c10::cuda::CUDAGuard guard(dev);
+    const int64_t s[3] = {B, H, c.head_dim};
+    int64_t bytes = 0;
+    ok(blk_paged_attention_workspace(&c, H, B, table.size(1), &bytes));
+    Tensor out = at::detail::empty_cuda(at::IntArrayRef(s, 3), q.scalar_type(), dev, std::nullopt);
+    if (lse) *lse = empty2(B, H, at::kFloat, dev);
+    if (B == 0) return out;
+    const Tensor work = at::detail::empty_cuda(at::IntArrayRef(&bytes, 1), at::kByte, dev, std::nullopt);
+    ok(blk_paged_attention(&c, q.data_ptr(), q.stride(0), q.stride(1), H, static_cast<const int32_t*>(table.data_ptr()), table.stride(0),
+                           table.size(1), static_cast<const int32_t*>(lengths.data_ptr()), B, (float)scale, out.data_ptr(),
+                           lse ? static_cast<float*>(lse->data_ptr()) : nullptr, work.data_ptr(), bytes, stream_of(dev)));
+    return out;
+}
+// paged_attention(q, kCache, vCache, pageTable, lengths, scale)
+Tensor py_paged_attention(PyObject* const* a) { return paged_attention(a, nullptr); }
+// paged_attention_lse(...) -> (out, lse)
+PyObject* py_paged_attention_lse(PyObject* const* a) {
+    Tensor lse;
+    const Tensor out = paged_attention(a, &lse);
+    PyRef x(THPVariable_Wrap(out)), y(THPVariable_Wrap(lse));
+    return x.o && y.o ? PyTuple_Pack(2, x.o, y.o) : nullptr;
+}
+
 // ---- the module --------------------------------------------------------------------------------------
+// Operators with other results than one tensor, or that write to their arguments, have no place in a trace.
+template <PyObject* (*F)(PyObject* const*), int NARGS>
+PyObject* entry_untraced(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == NARGS, "expected ", NARGS, " arguments");
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), "torch.jit.trace cannot record this operator");
+    return F(args);
+    END_HANDLE_TH_ERRORS
+}
+
 // F takes NARGS arguments, the first NTENSORS of them its operands.  torch.jit.trace sees nothing of what happens here: a
 // call that it is to record goes to apply.py and comes back, with the tracer paused, from a torch.autograd.Function.
 template <Tensor (*F)(PyObject* const*), const char* NAME, int NARGS, int NTENSORS>
@@ -975,14 +1120,21 @@ PyObject* py_setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define BLK_ENTRY(name, nargs, ntensors) \
     {g_##name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<py_##name, g_##name, nargs, ntensors>)), METH_FASTCALL, nullptr}
+#define BLK_ENTRY_UNTRACED(name, nargs) \
+    {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry_untraced<py_##name, nargs>)), METH_FASTCALL, nullptr}
 constexpr char g_gemm[] = "gemm", g_softmax[] = "softmax", g_attention[] = "attention",
-               g_attention_token_major[] = "attention_token_major", g_scores_token_major[] = "scores_token_major";
+               g_attention_token_major[] = "attention_token_major", g_scores_token_major[] = "scores_token_major",
+               g_paged_attention[] = "paged_attention";
 PyMethodDef g_methods[] = {
     BLK_ENTRY(gemm, 13, 2),
     BLK_ENTRY(softmax, 6, 1),
     BLK_ENTRY(attention, 7, 3),
     BLK_ENTRY(attention_token_major, 5, 3),
     BLK_ENTRY(scores_token_major, 6, 2),
+    BLK_ENTRY(paged_attention, 6, 5),
+    BLK_ENTRY_UNTRACED(paged_attention_lse, 6),
+    BLK_ENTRY_UNTRACED(paged_slots, 8),
+    BLK_ENTRY_UNTRACED(paged_append, 5),
     {"clear", py_clear, METH_NOARGS, nullptr},
     {"check", py_check, METH_NOARGS, nullptr},
     {"cached", py_cached, METH_NOARGS, nullptr},

@@ -238,6 +238,58 @@ BLK_API int blk_softmax_backward_run(const blk_plan_t* plan, const void* out, co
 BLK_API int blk_softmax_noalloc(const void* src, void* out, const int64_t* rows, const int64_t* cols,
                         int64_t S, int64_t H, int dtype, float scale, void* cuda_stream);
 
+/* ---- paged cache ------------------------------------------------------------ */
+
+/* Keys and values that are kept: pages of page_size tokens, in any order.  The row (head_dim elements) of token t of head h
+ * of page g starts at element g * page_stride + h * head_stride + t * token_stride of k, and of v.  k, v: dev pointers,
+ * 16-byte aligned; strides in elements, each row on a 16-byte boundary.  A request's tokens lie in the pages that its row of a page table
+ * names: token p on place p % page_size of page table[p / page_size].  The calls below run on the current device, need no plan,
+ * read no length or table on the host, neither allocate nor synchronise, and may be captured.  They have no
+ * counterpart in the upstream project, which keeps nothing between calls. */
+typedef struct {
+    void* k;
+    void* v;
+    int64_t pages;       /* at most 2^31 - 1 */
+    int64_t page_size;   /* 1 .. 2^30 */
+    int64_t heads;
+    int64_t head_dim;
+    int64_t page_stride, head_stride, token_stride;
+    int dtype;           /* blk_dtype_t */
+} blk_paged_cache_t;
+
+/* Pages and slots for new tokens.  Request r holds lengths[r] tokens and gets new_tokens[r] (dev; a negative number counts as
+ * zero).  Where they need pages beyond those it has (ceil(lengths[r] / page_size)), these are taken from free_pages (dev, num_free
+ * entries), from entry taken[0] on, request by request, and entered into its row of page_table (dev, rows of `columns` entries
+ * table_stride entries apart).  slots[i] (dev, `tokens` entries): page * page_size + place of the i-th new token, counted
+ * over all requests in order; -1 for one without a page (free_pages used up or negative, table row full) and behind the last
+ * one.  lengths_out[r] = lengths[r] + new_tokens[r]; taken_out[0] = pages asked for so far (more than num_free: they ran out).
+ * lengths_out may be lengths itself, taken_out taken; otherwise they must not overlap what is read. */
+BLK_API int blk_paged_slots(const int32_t* lengths, const int32_t* new_tokens, int64_t requests, int32_t* page_table,
+                            int64_t table_stride, int64_t columns, const int32_t* free_pages, int64_t num_free,
+                            const int32_t* taken, int64_t page_size, int64_t* slots, int64_t tokens, int32_t* lengths_out,
+                            int32_t* taken_out, void* cuda_stream);
+
+/* Row h of token i (k[i * k_row_stride + h * k_head_stride ...], v likewise; dev, 16-byte aligned rows of the cache's type) goes to
+ * slot slots[i] (dev) of head h.  Slots outside [0, pages * page_size) are passed over.  No slot may be given twice (its row would
+ * hold parts of both); rows of the cache must not overlap. */
+BLK_API int blk_paged_append(const blk_paged_cache_t* cache, const void* k, int64_t k_row_stride, int64_t k_head_stride,
+                             const void* v, int64_t v_row_stride, int64_t v_head_stride, const int64_t* slots, int64_t tokens,
+                             void* cuda_stream);
+
+/* out[r, h] = softmax(scale * q[r, h] K^T) V over the tokens that request r keeps of head h / (heads / cache heads): the first
+ * lengths[r] (no more than columns * page_size) but for those whose page_table entry is no page (negative, or
+ * >= pages).  A request without tokens gets zeros.  q: (requests, heads, head_dim) with the given strides in
+ * elements, rows on 16-byte boundaries; out: the same, packed; lse: natural logarithm of each row's softmax denominator,
+ * scale and maximum included (requests x heads floats, -inf without tokens), or NULL.  head_dim at most 256; heads a
+ * multiple of the cache's.  workspace: dev, 16-byte aligned, at least what blk_paged_attention_workspace says for the same arguments on
+ * the same device; calls that may overlap need one each. */
+BLK_API int blk_paged_attention_workspace(const blk_paged_cache_t* cache, int64_t heads, int64_t requests, int64_t columns,
+                                          int64_t* bytes);
+BLK_API int blk_paged_attention(const blk_paged_cache_t* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                                int64_t heads, const int32_t* page_table, int64_t table_stride, int64_t columns,
+                                const int32_t* lengths, int64_t requests, float scale, void* out, float* lse, void* workspace,
+                                int64_t workspace_bytes, void* cuda_stream);
+
 /* ---- plan queries ---------------------------------------------------------- */
 
 BLK_API void blk_plan_destroy(blk_plan_t* plan);
