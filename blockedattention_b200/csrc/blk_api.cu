@@ -1234,7 +1234,8 @@ extern "C" int blk_paged_attention(const blk_paged_cache_t* c, const void* q, in
     p.requests = (int)requests;
     p.q_units = s.q_units;
     p.rows_unit = s.rows_unit;
-    p.units = (int)c->heads * s.q_units;
+    p.kv_heads = (int)c->heads;
+    p.units = p.kv_heads * s.q_units;
     p.heads = (int)heads;
     p.d = (int)c->head_dim;
     p.pages = (int)c->pages;

@@ -278,7 +278,7 @@ struct BlkPagedAttnParams {
     int64_t table_stride;  // entries
     const int* lengths;
     int capacity;          // tokens that a row of the table has pages for
-    int requests, units, q_units, rows_unit, group, heads, d, pages;
+    int requests, kv_heads, units, q_units, rows_unit, group, heads, d, pages;  // units: of a request, kv_heads x q_units
     BlkDivisor page;
     void* out;
     float* lse;

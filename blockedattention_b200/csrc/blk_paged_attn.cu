@@ -17,7 +17,10 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_or_zeros(uint32_t dst, const void* src, bool there) {
     const int n = there ? 16 : 0;  // 0: sixteen zeros, nothing is read
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
@@ -41,6 +44,10 @@ __device__ __forceinline__ float part_weight(float m, float top, float c) {
     if (m == -INFINITY) return top == -INFINITY ? 1.f : 0.f;
     return blk_exp2((m - top) * c);
 }
+
+// Place of a column of row q among eight rows of DP floats: rows two apart lie eight banks apart, as a warp's accumulators are spread.
+template <int DP>
+__device__ __forceinline__ int merge_at(int q, int col) { return q * DP + (col ^ ((q >> 1) << 3)); }
 
 // ---- the arithmetic of one warp, 16-bit types ---------------------------------------------------------
 // Scores and values on the tensor cores with the tokens as the wide side: S^T = K Q^T is (16 tokens x 8 query rows), O^T = V^T P^T is
@@ -194,7 +201,7 @@ struct Math16 {
                 }
             }
     }
-    // this warp's weighted values of query rows 8n .. 8n+7, rows of DP + 4 floats; w: the rows' weights
+    // this warp's weighted values of query rows 8n .. 8n+7; w: the rows' weights
     __device__ __forceinline__ void put(int n_, float* dst, const float* w, int lane) {
         const int q = (lane & 3) * 2;
 #pragma unroll
@@ -203,11 +210,11 @@ struct Math16 {
                 const float w0 = w[n * 8 + q] * (1.f / PSplit<Tag>::SCALE), w1 = w[n * 8 + q + 1] * (1.f / PSplit<Tag>::SCALE);
 #pragma unroll
                 for (int mm = 0; mm < DP / 16; ++mm) {
-                    float* at = dst + q * (DP + 4) + mm * 16 + lane / 4;
-                    at[0] = o[mm][n][0] * w0;
-                    at[DP + 4] = o[mm][n][1] * w1;
-                    at[8] = o[mm][n][2] * w0;
-                    at[DP + 4 + 8] = o[mm][n][3] * w1;
+                    const int col = mm * 16 + lane / 4;
+                    dst[merge_at<DP>(q, col)] = o[mm][n][0] * w0;
+                    dst[merge_at<DP>(q + 1, col)] = o[mm][n][1] * w1;
+                    dst[merge_at<DP>(q, col + 8)] = o[mm][n][2] * w0;
+                    dst[merge_at<DP>(q + 1, col + 8)] = o[mm][n][3] * w1;
                 }
             }
     }
@@ -328,7 +335,7 @@ struct Math32 {
 #pragma unroll
             for (int j = 0; j < W; ++j) {
                 const int col = W == 2 ? lane * 2 + j : (j / 4) * 128 + lane * 4 + (j & 3);
-                dst[i * (DP + 4) + col] = o[i][j] * x;
+                dst[merge_at<DP>(i, col)] = o[i][j] * x;
             }
         }
     }
@@ -340,16 +347,16 @@ struct Lay {
     static constexpr int TILE = WARPS * M::TW;
     static constexpr int HALF = M::TW * M::RB;                       // a warp's keys, or values, of a stage
     static constexpr int RING = WARPS * M::STAGES * 2 * HALF;
-    static constexpr int MERGE = WARPS * 8 * (M::DP + 4) * 4;
+    static constexpr int MERGE = WARPS * 8 * M::DP * 4;
     static constexpr int STATS = (3 * WARPS + 2) * M::GU * 4;        // maxima, sums, weights of the warps; those of the block
     static constexpr int MASKS = WARPS * M::STAGES * 4;
-    static constexpr int SCHED = 64;
-    static constexpr int BYTES = RING + MERGE + M::EXTRA + STATS + MASKS + SCHED;
+    static constexpr int BYTES = RING + MERGE + M::EXTRA + STATS + MASKS;
+    static_assert((BYTES + 1024) * M::CTAS <= 228 * 1024, "the blocks that a kernel is made for fit on an SM");
 };
 
-// Where a block is in the list of tiles: tile t of n of unit u (a key head, or a part of its query rows) of request r.
+// Where a block is in the list of tiles: tile t of n, of part `part` of the query rows of key head `kv`, of request r.
 struct Walk {
-    int r, u, t, n, len, ahead;
+    int r, kv, part, t, n, len, ahead;
 };
 __device__ __forceinline__ int held(const BlkPagedAttnParams& p, int r) {
     return min(max(p.lengths[r], 0), p.capacity);
@@ -360,8 +367,10 @@ template <int TILE>
 __device__ __forceinline__ void step(Walk& w, const BlkPagedAttnParams& p) {
     if (++w.t < w.n) return;
     w.t = 0;
-    if (++w.u < p.units) return;
-    w.u = 0;
+    if (++w.part < p.q_units) return;
+    w.part = 0;
+    if (++w.kv < p.kv_heads) return;
+    w.kv = 0;
     ++w.r;
     w.len = w.ahead;
     w.n = tiles_of<TILE>(w.len);
@@ -402,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     float* const top_m = sm_w + WARPS * GU;
     float* const top_l = top_m + GU;
     uint32_t* const masks = reinterpret_cast<uint32_t*>(top_l + GU) + threadIdx.x / 32 * STAGES;
-    int64_t* const sched = reinterpret_cast<int64_t*>(smem + L::RING + L::MERGE + M::EXTRA + L::STATS + L::MASKS);
+    int64_t* const sched = reinterpret_cast<int64_t*>(merge);  // (up to the first merge)
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const uint32_t ring = blk_smem_u32(smem) + warp * (STAGES * 2 * L::HALF), extra = blk_smem_u32(smem) + L::RING + L::MERGE;
     const int chunks = p.d * M::E / 16;
@@ -415,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
 
     // The lengths, added up: a run of requests for every thread.
     Walk cw;
-    int64_t lo, hi;
+    int64_t lo, hi, all = 0, blocks;
     {
         const int per = (p.requests + THREADS - 1) / THREADS, r0 = min(tid * per, p.requests), r1 = min(r0 + per, p.requests);
         int64_t mine = 0;
@@ -428,7 +437,6 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         }
         if (lane == 31) sched[warp] = before;
         __syncthreads();
-        int64_t all = 0;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             if (w < warp) before += sched[w];
@@ -436,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         }
         before -= mine;
         all *= p.units;
-        const int64_t blocks = min((int64_t)gridDim.x, all);
+        blocks = min((int64_t)gridDim.x, all);
         if (blockIdx.x >= blocks) {
             if (tid == 0) p.parts[blockIdx.x] = make_int4(0, 0, 0, 0);
             return;
@@ -455,21 +463,20 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
             sched[4] = r;
             sched[5] = lo - at * p.units;
         }
-        if (tid == 0) {
-            sched[6] = all;
-            sched[7] = blocks;
-        }
         __syncthreads();
         cw.r = (int)sched[4];
         cw.len = held(p, cw.r);
         cw.n = tiles_of<TILE>(cw.len);
-        cw.u = (int)(sched[5] / cw.n);
+        const int unit = (int)(sched[5] / cw.n);
         cw.t = (int)(sched[5] % cw.n);
+        cw.kv = unit / p.q_units;
+        cw.part = unit % p.q_units;
         cw.ahead = cw.r + 1 < p.requests ? held(p, cw.r + 1) : 0;
     }
     const int64_t count = hi - lo;
 
-    // Copies.  A lane looks up the page of one of the warp's tokens, a tile before its rows are asked for.
+    // Copies.  A lane looks up the page of one of the warp's tokens, a tile before its rows are asked for; eight lanes take 128
+    // bytes of a row.
     Walk pw = cw;
     int entry = -1;
     int64_t inner = 0;
@@ -479,27 +486,30 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         if (lane < TW && tok < (unsigned)pw.len) {
             const unsigned col = (__umulhi(tok, p.page.magic) + tok) >> p.page.shift;
             entry = p.table[pw.r * p.table_stride + col];
-            inner = (int64_t)(tok - col * p.page.d) * p.token_stride + (int64_t)(pw.u / p.q_units) * p.head_stride;
+            inner = (int64_t)(tok - col * p.page.d) * p.token_stride + pw.kv * p.head_stride;
         }
     };
+    const int piece = lane & 7, row8 = lane >> 3;
     auto load = [&](int stage) {
         const bool there = entry >= 0 && entry < p.pages;
         const int64_t off = there ? entry * p.page_stride + inner : -1;
         const uint32_t mask = __ballot_sync(0xffffffffu, there);
         if (lane == 0) masks[stage] = mask;
-        if (mask) {
-            const uint32_t sK = ring + stage * (2 * L::HALF), sV = sK + L::HALF;
+        if (!mask) return;
+        const uint32_t to = ring + stage * (2 * L::HALF);
 #pragma unroll
-            for (int i = 0; i < TW * CPR / 32; ++i) {
-                const int idx = i * 32 + lane, row = idx / CPR, ch = idx % CPR;
-                const int64_t o = __shfl_sync(0xffffffffu, off, row);
-                if (ch < chunks) {
-                    const int64_t at = (o < 0 ? 0 : o) + ch * 16;
-                    const uint32_t dst = row * RB + ((ch ^ (row & 7)) << 4);
-                    if (o >= 0) cp_async16(sK + dst, p.k + at, true);
-                    cp_async16(sV + dst, p.v + at, o >= 0);
+        for (int i = 0; i < TW / 4; ++i) {
+            const int row = i * 4 + row8;
+            const int64_t o = __shfl_sync(0xffffffffu, off, row);
+            const bool have = o >= 0;
+            const char *const k = p.k + (have ? o : 0) + piece * 16, *const v = p.v + (have ? o : 0) + piece * 16;
+            const uint32_t dst = to + row * RB + ((piece ^ (row & 7)) << 4);
+#pragma unroll
+            for (int j = 0; j < CPR / 8; ++j)
+                if (piece + 8 * j < chunks) {
+                    if (have) cp_async16(dst + 128 * j, k + 128 * j);
+                    cp_async16_or_zeros(dst + L::HALF + 128 * j, v + 128 * j, have);  // (a weight of zero times what lies there)
                 }
-            }
         }
     };
     look();
@@ -520,12 +530,15 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     for (int s = 0; s < STAGES - 1; ++s) next();
 
     M math;
-    int stage = 0, part_of = 0;
+    int stage = 0, first = 0, rows = 0, head0 = 0;
     int4 part = make_int4(0, 0, 0, 0);
     for (int64_t i = 0; i < count; ++i) {
-        const int kv = cw.u / p.q_units, first = (cw.u % p.q_units) * p.rows_unit, rows = min(p.rows_unit, p.group - first);
-        const int64_t head0 = (int64_t)kv * p.group + first;
-        if (i == 0 || cw.t == 0) math.begin(p, p.q + cw.r * p.q_row_stride + head0 * p.q_head_stride, rows, extra, lane);
+        if (i == 0 || cw.t == 0) {
+            first = cw.part * p.rows_unit;
+            rows = min(p.rows_unit, p.group - first);
+            head0 = cw.kv * p.group + first;
+            math.begin(p, p.q + cw.r * p.q_row_stride + head0 * p.q_head_stride, rows, extra, lane);
+        }
         cp_wait<STAGES - 2>();
         __syncwarp();
         next();
@@ -558,15 +571,15 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
             float* const ws = p.work + (int64_t)slot * (GU * DP + 2 * GU);
 #pragma unroll 1
             for (int n = 0; n < M::NT; ++n) {
-                math.put(n, merge + warp * (8 * (DP + 4)), sm_w + warp * GU, lane);
+                math.put(n, merge + warp * (8 * DP), sm_w + warp * GU, lane);
                 __syncthreads();
                 for (int x = tid; x < 8 * DP / 4; x += THREADS) {
                     const int q = x / (DP / 4), col = x % (DP / 4) * 4, row = n * 8 + q;
                     if (row >= rows || col >= p.d) continue;
-                    float4 v = *reinterpret_cast<const float4*>(merge + q * (DP + 4) + col);
+                    float4 v = *reinterpret_cast<const float4*>(merge + merge_at<DP>(q, col));
 #pragma unroll
                     for (int w = 1; w < WARPS; ++w) {
-                        const float4 y = *reinterpret_cast<const float4*>(merge + (w * 8 + q) * (DP + 4) + col);
+                        const float4 y = *reinterpret_cast<const float4*>(merge + w * (8 * DP) + merge_at<DP>(q, col));
                         v.x += y.x;
                         v.y += y.y;
                         v.z += y.z;
@@ -588,8 +601,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
             }
             if (begins && !ends) {  // the head goes on in the blocks up to the one that has its last tile
                 const int64_t last = lo + i - cw.t + cw.n - 1;
-                part_of = (int)(((last + 1) * sched[7] - 1) / sched[6]) - (int)blockIdx.x + 1;
-                part = make_int4(part_of, cw.r, cw.u, 0);
+                part = make_int4((int)(((last + 1) * blocks - 1) / all) - (int)blockIdx.x + 1, cw.r, cw.kv, cw.part);
             }
         }
         if (i + 1 < count) step<TILE>(cw, p);
@@ -608,7 +620,7 @@ __global__ void __launch_bounds__(512) blk_paged_join_kernel(const BlkPagedAttnP
     const int4 part = p.parts[blockIdx.x];
     const int n = part.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, sub = warp / 4, row = blockIdx.y * 4 + warp % 4;
     if (n == 0) return;
-    const int kv = part.z / p.q_units, first = (part.z % p.q_units) * p.rows_unit, rows = min(p.rows_unit, p.group - first);
+    const int kv = part.z, first = part.w * p.rows_unit, rows = min(p.rows_unit, p.group - first);
     if ((int)blockIdx.y * 4 >= rows) return;
     const bool mine = row < rows;
     const int64_t size = GU * DP + 2 * GU;
