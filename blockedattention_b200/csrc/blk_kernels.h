@@ -285,7 +285,7 @@ struct BlkPagedAttnParams {
     float* work;
     int4* parts;
     float c, scale;        // |scale| log2(e), |scale|
-    int negate;            // scale < 0: the kernel takes -q
+    float sign;            // of the scale
 };
 // How a call is cut: padded head dimension, units a key head's query rows are taken in, their rows and eights of rows,
 // blocks, and what these leave for the join.

@@ -39,11 +39,10 @@ __device__ __forceinline__ float4 lds128(uint32_t addr) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
 }
-// Weight of a part whose maximum is m where the whole's is top.  -inf: the part saw nothing, or scores of -inf alone.
-__device__ __forceinline__ float part_weight(float m, float top, float c) {
-    if (m == -INFINITY) return top == -INFINITY ? 1.f : 0.f;
-    return blk_exp2((m - top) * c);
-}
+// A part of a row: maximum m and sum l of its weights relative to m.  l = 0: it saw no token, and its values are not there.
+// l = inf, m = -inf: it saw scores of -inf alone, which count only where every part is like that (0 / 0).  A NaN in l is kept.
+__device__ __forceinline__ bool part_counts(float l, float top) { return l != 0.f && !(l == INFINITY && top > -INFINITY); }
+__device__ __forceinline__ float part_weight(float m, float top, float c) { return m == -INFINITY ? 1.f : blk_exp2((m - top) * c); }
 
 // Place of a column of row q among eight rows of DP floats: rows two apart lie eight banks apart, as a warp's accumulators are spread.
 template <int DP>
@@ -86,8 +85,8 @@ struct Math16 {
     float m[NT][2], l[NT][2];
     bool seen;
 
-    __device__ __forceinline__ void begin(const BlkPagedAttnParams& p, const char* q, int rows, uint32_t, int lane) {
-        const uint32_t flip = p.negate ? 0x80008000u : 0u;
+    // q on its way: nothing here waits for it
+    __device__ __forceinline__ void fetch(const BlkPagedAttnParams& p, const char* q, int rows, int lane) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int row = n * 8 + lane / 4;
@@ -97,8 +96,13 @@ struct Math16 {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int col = kk * 16 + h * 8;
-                    qf[kk][n][h] = row < rows && col < p.d ? *reinterpret_cast<const uint32_t*>(at + col * 2) ^ flip : 0u;
+                    qf[kk][n][h] = row < rows && col < p.d ? *reinterpret_cast<const uint32_t*>(at + col * 2) : 0u;
                 }
+        }
+    }
+    __device__ __forceinline__ void begin(uint32_t) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
             m[n][0] = m[n][1] = -INFINITY;
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
@@ -109,13 +113,16 @@ struct Math16 {
         seen = false;
     }
 
-    __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float c, uint32_t, int lane) {
+    __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float sign, float c, uint32_t, int lane) {
+        constexpr int CHAINS = NT == 1 ? 2 : 1;  // sums that do not wait for one another
         seen = true;
-        float s[NT][4];
+        float s[NT][4], part[CHAINS][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < CHAINS; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[i][n][e] = 0.f;
         {
             const int row = lane & 15;
             const uint32_t base = sK + row * RB, x = ((lane >> 4) ^ (row & 7)) << 4;
@@ -124,9 +131,13 @@ struct Math16 {
                 uint32_t a[4];
                 blk_ldmatrix_x4(a, base + ((kk * 32) ^ x));
 #pragma unroll
-                for (int n = 0; n < NT; ++n) blk_mma16816<Tag>(s[n], a[0], a[1], a[2], a[3], qf[kk][n][0], qf[kk][n][1]);
+                for (int n = 0; n < NT; ++n) blk_mma16816<Tag>(part[kk % CHAINS][n], a[0], a[1], a[2], a[3], qf[kk][n][0], qf[kk][n][1]);
             }
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = (CHAINS == 2 ? part[0][n][e] + part[CHAINS - 1][n][e] : part[0][n][e]) * sign;
         const bool v0 = mask >> (lane / 4) & 1, v1 = mask >> (lane / 4 + 8) & 1;
         uint32_t hi[NT][2], lo[NT][2];
         float alpha[NT][2];
@@ -197,27 +208,27 @@ struct Math16 {
                 t += __shfl_xor_sync(0xffffffffu, t, 16);
                 if (lane < 4) {
                     sm[n * 8 + lane * 2 + e] = m[n][e];
-                    sl[n * 8 + lane * 2 + e] = seen && m[n][e] == -INFINITY ? NAN : t;  // scores of -inf alone: 0 / 0
+                    sl[n * 8 + lane * 2 + e] = seen && t == 0.f ? INFINITY : t;
                 }
             }
     }
-    // this warp's weighted values of query rows 8n .. 8n+7; w: the rows' weights
-    __device__ __forceinline__ void put(int n_, float* dst, const float* w, int lane) {
+    // this warp's values of query rows 8n .. 8n+7, relative to its own maxima; rows: how many of all rows there are
+    __device__ __forceinline__ void put(int n_, float* dst, int rows, int lane) {
         const int q = (lane & 3) * 2;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-            if (n == n_) {
-                const float w0 = w[n * 8 + q] * (1.f / PSplit<Tag>::SCALE), w1 = w[n * 8 + q + 1] * (1.f / PSplit<Tag>::SCALE);
+            if (n == n_ && n * 8 + q < rows) {
 #pragma unroll
                 for (int mm = 0; mm < DP / 16; ++mm) {
                     const int col = mm * 16 + lane / 4;
-                    dst[merge_at<DP>(q, col)] = o[mm][n][0] * w0;
-                    dst[merge_at<DP>(q + 1, col)] = o[mm][n][1] * w1;
-                    dst[merge_at<DP>(q, col + 8)] = o[mm][n][2] * w0;
-                    dst[merge_at<DP>(q + 1, col + 8)] = o[mm][n][3] * w1;
+                    dst[merge_at<DP>(q, col)] = o[mm][n][0];
+                    dst[merge_at<DP>(q + 1, col)] = o[mm][n][1];
+                    dst[merge_at<DP>(q, col + 8)] = o[mm][n][2];
+                    dst[merge_at<DP>(q + 1, col + 8)] = o[mm][n][3];
                 }
             }
     }
+    static constexpr float OUT_SCALE = 1.f / PSplit<Tag>::SCALE;
 };
 
 // ---- the same in 32 bits -------------------------------------------------------------------------------
@@ -233,12 +244,18 @@ struct Math32 {
     float m[8], l[8];
     bool seen;
 
-    __device__ __forceinline__ void begin(const BlkPagedAttnParams& p, const char* q, int rows, uint32_t sx, int) {
-        for (int i = threadIdx.x; i < 8 * DP; i += THREADS) {
-            const int row = i / DP, col = i % DP;
-            float v = row < rows && col < p.d ? reinterpret_cast<const float*>(q + row * p.q_head_stride)[col] : 0.f;
-            blk_sts_f32(sx + i * 4, p.negate ? -v : v);
+    float qv[8 * DP / THREADS];
+    __device__ __forceinline__ void fetch(const BlkPagedAttnParams& p, const char* q, int rows, int) {
+#pragma unroll
+        for (int j = 0; j < 8 * DP / THREADS; ++j) {
+            const int i = j * THREADS + threadIdx.x, row = i / DP, col = i % DP;
+            qv[j] = row < rows && col < p.d ? reinterpret_cast<const float*>(q + row * p.q_head_stride)[col] : 0.f;
         }
+    }
+    // (behind a barrier that no warp reaches before its last tile of the head before)
+    __device__ __forceinline__ void begin(uint32_t sx) {
+#pragma unroll
+        for (int j = 0; j < 8 * DP / THREADS; ++j) blk_sts_f32(sx + (j * THREADS + threadIdx.x) * 4, qv[j]);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -250,7 +267,7 @@ struct Math32 {
         seen = false;
     }
 
-    __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float c, uint32_t sx, int lane) {
+    __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float sign, float c, uint32_t sx, int lane) {
         seen = true;
         const int tok = lane % TW, part = lane / TW;
         const bool valid = mask >> tok & 1;
@@ -273,6 +290,7 @@ struct Math32 {
         for (int i = 0; i < 8; ++i) {
 #pragma unroll
             for (int x = TW; x < 32; x *= 2) s[i] += __shfl_xor_sync(0xffffffffu, s[i], x);
+            s[i] *= sign;
             float t = valid ? s[i] : -INFINITY;
 #pragma unroll
             for (int x = 1; x < TW; x *= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
@@ -324,21 +342,22 @@ struct Math32 {
             for (int x = 1; x < TW; x *= 2) t += __shfl_xor_sync(0xffffffffu, t, x);
             if (lane == 0) {
                 sm[i] = m[i];
-                sl[i] = seen && m[i] == -INFINITY ? NAN : t;
+                sl[i] = seen && t == 0.f ? INFINITY : t;
             }
         }
     }
-    __device__ __forceinline__ void put(int, float* dst, const float* w, int lane) {
+    __device__ __forceinline__ void put(int, float* dst, int rows, int lane) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = w[i];
+        for (int i = 0; i < 8; ++i)
+            if (i < rows) {
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const int col = W == 2 ? lane * 2 + j : (j / 4) * 128 + lane * 4 + (j & 3);
-                dst[merge_at<DP>(i, col)] = o[i][j] * x;
+                for (int j = 0; j < W; ++j) {
+                    const int col = W == 2 ? lane * 2 + j : (j / 4) * 128 + lane * 4 + (j & 3);
+                    dst[merge_at<DP>(i, col)] = o[i][j];
+                }
             }
-        }
     }
+    static constexpr float OUT_SCALE = 1.f;
 };
 
 // ---- shared memory -------------------------------------------------------------------------------------
@@ -348,7 +367,7 @@ struct Lay {
     static constexpr int HALF = M::TW * M::RB;                       // a warp's keys, or values, of a stage
     static constexpr int RING = WARPS * M::STAGES * 2 * HALF;
     static constexpr int MERGE = WARPS * 8 * M::DP * 4;
-    static constexpr int STATS = (3 * WARPS + 2) * M::GU * 4;        // maxima, sums, weights of the warps; those of the block
+    static constexpr int STATS = 2 * WARPS * M::GU * 4;              // maxima and sums of the warps
     static constexpr int MASKS = WARPS * M::STAGES * 4;
     static constexpr int BYTES = RING + MERGE + M::EXTRA + STATS + MASKS;
     static_assert((BYTES + 1024) * M::CTAS <= 228 * 1024, "the blocks that a kernel is made for fit on an SM");
@@ -392,12 +411,14 @@ template <> struct Out<BlkFloatTag> {
     static __device__ __forceinline__ void put4(void* out, int64_t at, float4 v) { *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v; }
 };
 
-// Result of a head's row from its sum and weighted values.  No token at all: l = 0 and zeros.
-__device__ __forceinline__ float4 divided(float4 v, float l) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+// Result of a head's row from its sum and weighted values.  No token at all: l = 0 and zeros; scores of -inf alone: l = inf and NaN.
+__device__ __forceinline__ float4 divided(float4 v, float l, float scale) {
+    const float inv = l == 0.f ? 0.f : l == INFINITY ? NAN : scale / l;
     return make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
 }
 __device__ __forceinline__ float row_log(float m, float l, float scale) { return l == 0.f ? -INFINITY : m * scale + logf(l); }
+
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (a | b) >> 32 ? a / b : (unsigned)a / (unsigned)b; }
 
 template <typename M>
 __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const BlkPagedAttnParams p) {
@@ -407,10 +428,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     float* const merge = reinterpret_cast<float*>(smem + L::RING);
     float* const sm_m = reinterpret_cast<float*>(smem + L::RING + L::MERGE + M::EXTRA);
     float* const sm_l = sm_m + WARPS * GU;
-    float* const sm_w = sm_l + WARPS * GU;
-    float* const top_m = sm_w + WARPS * GU;
-    float* const top_l = top_m + GU;
-    uint32_t* const masks = reinterpret_cast<uint32_t*>(top_l + GU) + threadIdx.x / 32 * STAGES;
+    uint32_t* const masks = reinterpret_cast<uint32_t*>(sm_l + WARPS * GU) + threadIdx.x / 32 * STAGES;
     int64_t* const sched = reinterpret_cast<int64_t*>(merge);  // (up to the first merge)
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const uint32_t ring = blk_smem_u32(smem) + warp * (STAGES * 2 * L::HALF), extra = blk_smem_u32(smem) + L::RING + L::MERGE;
@@ -449,44 +467,50 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
             if (tid == 0) p.parts[blockIdx.x] = make_int4(0, 0, 0, 0);
             return;
         }
-        lo = blockIdx.x * all / blocks;
-        hi = (blockIdx.x + 1) * all / blocks;
-        const int64_t x = lo / p.units;
+        lo = quotient(blockIdx.x * all, blocks);
+        hi = quotient((blockIdx.x + 1) * all, blocks);
+        const int64_t x = quotient(lo, p.units);
         if (x >= before && x < before + mine) {
             int r = r0;
             int64_t at = before;
-            int n = tiles_of<TILE>(held(p, r));
+            int len = held(p, r), n = tiles_of<TILE>(len);
             while (x >= at + n) {
                 at += n;
-                n = tiles_of<TILE>(held(p, ++r));
+                len = held(p, ++r);
+                n = tiles_of<TILE>(len);
             }
             sched[4] = r;
             sched[5] = lo - at * p.units;
+            sched[6] = len;
         }
         __syncthreads();
         cw.r = (int)sched[4];
-        cw.len = held(p, cw.r);
-        cw.n = tiles_of<TILE>(cw.len);
-        const int unit = (int)(sched[5] / cw.n);
-        cw.t = (int)(sched[5] % cw.n);
-        cw.kv = unit / p.q_units;
-        cw.part = unit % p.q_units;
         cw.ahead = cw.r + 1 < p.requests ? held(p, cw.r + 1) : 0;
+        cw.len = (int)sched[6];
+        cw.n = tiles_of<TILE>(cw.len);
+        const int unit = (int)quotient(sched[5], cw.n);
+        cw.t = (int)(sched[5] - (int64_t)unit * cw.n);
+        cw.kv = unit / p.q_units;
+        cw.part = unit - cw.kv * p.q_units;
     }
     const int64_t count = hi - lo;
 
-    // Copies.  A lane looks up the page of one of the warp's tokens, a tile before its rows are asked for; eight lanes take 128
+    // Copies.  A lane looks up the page of one of the warp's tokens, two tiles before its rows are asked for; eight lanes take 128
     // bytes of a row.
+    M math;
+    auto q_at = [&](const Walk& w) { return p.q + w.r * p.q_row_stride + (int64_t)(w.kv * p.group + w.part * p.rows_unit) * p.q_head_stride; };
+    auto rows_at = [&](const Walk& w) { return min(p.rows_unit, p.group - w.part * p.rows_unit); };
+    math.fetch(p, q_at(cw), rows_at(cw), lane);
     Walk pw = cw;
-    int entry = -1;
-    int64_t inner = 0;
+    int entry = -1, entry2 = -1;
+    int64_t inner = 0, inner2 = 0;
     auto look = [&]() {
         const unsigned tok = (unsigned)pw.t * TILE + warp * TW + lane;
-        entry = -1;
+        entry2 = -1;
         if (lane < TW && tok < (unsigned)pw.len) {
             const unsigned col = (__umulhi(tok, p.page.magic) + tok) >> p.page.shift;
-            entry = p.table[pw.r * p.table_stride + col];
-            inner = (int64_t)(tok - col * p.page.d) * p.token_stride + pw.kv * p.head_stride;
+            entry2 = p.table[pw.r * p.table_stride + col];
+            inner2 = (int64_t)(tok - col * p.page.d) * p.token_stride + pw.kv * p.head_stride;
         }
     };
     const int piece = lane & 7, row8 = lane >> 3;
@@ -512,99 +536,101 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
                 }
         }
     };
-    look();
     int64_t loaded = 0;
     int into = 0;
+    auto look_on = [&](int64_t i) {
+        entry = entry2;
+        inner = inner2;
+        if (i < count) {
+            step<TILE>(pw, p);
+            if (pw.t == 0 && warp == 0 && lane < rows_at(pw)) {  // a new head: its queries are wanted soon
+                const char* at = q_at(pw) + lane * p.q_head_stride;
+                for (int x = 0; x < p.d * M::E; x += 128) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(at + x));
+            }
+            look();
+        }
+    };
     auto next = [&]() {
         if (loaded < count) {
             load(into);
             into = into + 1 == STAGES ? 0 : into + 1;
-            if (++loaded < count) {
-                step<TILE>(pw, p);
-                look();
-            }
+            ++loaded;
+            look_on(loaded + 1);
         }
         cp_commit();
     };
+    look();
+    look_on(1);
 #pragma unroll 1
     for (int s = 0; s < STAGES - 1; ++s) next();
 
-    M math;
-    int stage = 0, first = 0, rows = 0, head0 = 0;
+    int stage = 0;
     int4 part = make_int4(0, 0, 0, 0);
+    math.begin(extra);
     for (int64_t i = 0; i < count; ++i) {
-        if (i == 0 || cw.t == 0) {
-            first = cw.part * p.rows_unit;
-            rows = min(p.rows_unit, p.group - first);
-            head0 = cw.kv * p.group + first;
-            math.begin(p, p.q + cw.r * p.q_row_stride + head0 * p.q_head_stride, rows, extra, lane);
-        }
         cp_wait<STAGES - 2>();
         __syncwarp();
         next();
         const uint32_t mask = masks[stage];
         if (mask) {
             const uint32_t sK = ring + stage * (2 * L::HALF);
-            math.tile(sK, sK + L::HALF, mask, p.c, extra, lane);
+            math.tile(sK, sK + L::HALF, mask, p.sign, p.c, extra, lane);
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
-        const bool ends = cw.t + 1 == cw.n;
-        if (ends || i + 1 == count) {
-            const bool begins = i >= cw.t;
-            math.stats(sm_m + warp * GU, sm_l + warp * GU, lane);
-            __syncthreads();
-            if (tid < GU) {
-                float top = sm_m[tid], sum = 0.f;
-#pragma unroll
-                for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w * GU + tid]);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float x = part_weight(sm_m[w * GU + tid], top, p.c);
-                    sm_w[w * GU + tid] = x;
-                    if (x != 0.f) sum += x * sm_l[w * GU + tid];
-                }
-                top_m[tid] = top;
-                top_l[tid] = sum;
-            }
-            __syncthreads();
-            const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
-            float* const ws = p.work + (int64_t)slot * (GU * DP + 2 * GU);
+        const bool ends = cw.t + 1 == cw.n, more = i + 1 < count;
+        const Walk now = cw;
+        if (more) step<TILE>(cw, p);
+        if (ends || !more) {
+            if (more) math.fetch(p, q_at(cw), rows_at(cw), lane);
+            const bool begins = i >= now.t;
+            const int first = now.part * p.rows_unit, rows = rows_at(now);
+            float* const ws = p.work + (2 * (int64_t)blockIdx.x + (begins ? 1 : 0)) * (GU * DP + 2 * GU);
+            const int64_t head0 = (int64_t)now.r * p.heads + now.kv * p.group + first;
 #pragma unroll 1
             for (int n = 0; n < M::NT; ++n) {
-                math.put(n, merge + warp * (8 * DP), sm_w + warp * GU, lane);
+                __syncthreads();  // (what was put here before is read)
+                if (n == 0) math.stats(sm_m + warp * GU, sm_l + warp * GU, lane);
+                if (math.seen) math.put(n, merge + warp * (8 * DP), rows, lane);
                 __syncthreads();
-                for (int x = tid; x < 8 * DP / 4; x += THREADS) {
+                const int here = min(8, rows - n * 8);
+                for (int x = tid; x < here * (DP / 4); x += THREADS) {
                     const int q = x / (DP / 4), col = x % (DP / 4) * 4, row = n * 8 + q;
-                    if (row >= rows || col >= p.d) continue;
-                    float4 v = *reinterpret_cast<const float4*>(merge + merge_at<DP>(q, col));
+                    if (col >= p.d) continue;
+                    float top = sm_m[row], l = 0.f;
 #pragma unroll
-                    for (int w = 1; w < WARPS; ++w) {
-                        const float4 y = *reinterpret_cast<const float4*>(merge + w * (8 * DP) + merge_at<DP>(q, col));
-                        v.x += y.x;
-                        v.y += y.y;
-                        v.z += y.z;
-                        v.w += y.w;
+                    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w * GU + row]);
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < WARPS; ++w) {
+                        const float lw = sm_l[w * GU + row], f = part_weight(sm_m[w * GU + row], top, p.c);
+                        if (part_counts(lw, top)) {
+                            const float4 y = *reinterpret_cast<const float4*>(merge + w * (8 * DP) + merge_at<DP>(q, col));
+                            l = fmaf(f, lw, l);
+                            v.x = fmaf(f, y.x, v.x);
+                            v.y = fmaf(f, y.y, v.y);
+                            v.z = fmaf(f, y.z, v.z);
+                            v.w = fmaf(f, y.w, v.w);
+                        }
                     }
                     if (begins && ends) {
-                        const int64_t head = (int64_t)cw.r * p.heads + head0 + row;
-                        Out<typename M::Tag>::put4(p.out, head * p.d + col, divided(v, top_l[row]));
-                        if (p.lse && col == 0) p.lse[head] = row_log(top_m[row], top_l[row], p.scale);
+                        const int64_t head = head0 + row;
+                        Out<typename M::Tag>::put4(p.out, head * p.d + col, divided(v, l, M::OUT_SCALE));
+                        if (p.lse && col == 0) p.lse[head] = row_log(top, l, p.scale);
                     } else {
                         *reinterpret_cast<float4*>(ws + row * DP + col) = v;
                         if (col == 0) {
-                            ws[GU * DP + row] = top_m[row];
-                            ws[GU * DP + GU + row] = top_l[row];
+                            ws[GU * DP + row] = top;
+                            ws[GU * DP + GU + row] = l;
                         }
                     }
                 }
-                __syncthreads();
             }
             if (begins && !ends) {  // the head goes on in the blocks up to the one that has its last tile
-                const int64_t last = lo + i - cw.t + cw.n - 1;
-                part = make_int4((int)(((last + 1) * blocks - 1) / all) - (int)blockIdx.x + 1, cw.r, cw.kv, cw.part);
+                const int64_t last = lo + i - now.t + now.n - 1;
+                part = make_int4((int)quotient((last + 1) * blocks - 1, all) - (int)blockIdx.x + 1, now.r, now.kv, now.part);
             }
+            if (more) math.begin(extra);
         }
-        if (i + 1 < count) step<TILE>(cw, p);
     }
     cp_wait<0>();
     if (tid == 0) p.parts[blockIdx.x] = part;
@@ -613,7 +639,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
 // Joins the parts of the heads that were cut: block (c, y) those of the head that begins in block c and goes on, four query rows
 // each, four warps to a row.
 template <typename Tag, int DP>
-__global__ void __launch_bounds__(512) blk_paged_join_kernel(const BlkPagedAttnParams p, int GU) {
+__global__ void __launch_bounds__(512) blk_paged_join_kernel(const BlkPagedAttnParams p, int GU, float out_scale) {
     __shared__ float sums[16][DP];
     __shared__ float denom[16];
     blk_grid_wait();
@@ -638,12 +664,12 @@ __global__ void __launch_bounds__(512) blk_paged_join_kernel(const BlkPagedAttnP
 #pragma unroll 4
         for (int i = sub; i < n; i += 4) {
             const float* a = at(i);
-            const float w = part_weight(a[GU * DP + row], top, p.c);
-            const float l = a[GU * DP + GU + row];
-            if (w != 0.f) sum += w * l;
+            const float l = a[GU * DP + GU + row], w = part_weight(a[GU * DP + row], top, p.c);
+            const bool counts = part_counts(l, top);
+            if (counts) sum = fmaf(w, l, sum);
 #pragma unroll
             for (int j = 0; j < DP / 32; ++j)
-                if (lane + 32 * j < p.d) acc[j] = fmaf(w, a[row * DP + lane + 32 * j], acc[j]);
+                if (counts && lane + 32 * j < p.d) acc[j] = fmaf(w, a[row * DP + lane + 32 * j], acc[j]);
         }
     }
 #pragma unroll
@@ -663,7 +689,7 @@ __global__ void __launch_bounds__(512) blk_paged_join_kernel(const BlkPagedAttnP
         v.w += y.w;
     }
     const int64_t head = (int64_t)part.y * p.heads + (int64_t)kv * p.group + first + row;
-    Out<Tag>::put4(p.out, head * p.d + col, divided(v, l));
+    Out<Tag>::put4(p.out, head * p.d + col, divided(v, l, out_scale));
     if (p.lse && col == 0) p.lse[head] = row_log(top, l, p.scale);
 }
 
@@ -735,6 +761,6 @@ cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedSha
         e = blk_launch(true, kern, dim3((unsigned)s.blocks), dim3(THREADS), (size_t)Lay<M>::BYTES, st, p);
         if (e != cudaSuccess || s.blocks == 1) return e;
         return blk_launch(true, blk_paged_join_kernel<typename M::Tag, M::DP>, dim3((unsigned)s.blocks, (unsigned)(s.rows_unit + 3) / 4), dim3(512),
-                          (size_t)0, st, p, GU);
+                          (size_t)0, st, p, GU, M::OUT_SCALE);
     });
 }

@@ -165,6 +165,24 @@ def test_infinities_and_nan_stay_in_their_rows(cuda_device, dtype):
     assert (out[5, 4:, 7] == math.inf).all() and torch.equal(out[5, 4:, :7], want[5, 4:, :7])
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n", [40, 300, 30000])
+def test_a_nan_is_not_lost_behind_large_scores(cuda_device, dtype, n):
+    """A key of NaN among scores that have no weight (e^-1000 of the largest), in another warp, block or part than the largest; and keys of
+    -inf alone there, which do have none."""
+    q, k, v, table, lengths = make([n, n, n], 1, 2, 64, 16, dtype)
+    q[:] = 1.0
+    k[:] = 0.0
+    k[table[:, 0].long(), 0, 0] = 16.0   # the first token's score: 1024
+    k[table[0, n // 16 - 1], 0, 5] = math.nan
+    k[table[1, 1:].long(), 0] = math.nan
+    k[table[2, 1:].long(), 0] = -math.inf
+    out, lse = blockPagedAttention(q, k, v, table, lengths, 1.0, return_lse=True)
+    assert torch.isnan(out[:2]).all() and torch.isnan(lse[:2]).all()
+    want = v[table[2, 0].long(), 0, 0].expand(2, -1)
+    assert torch.equal(out[2], want) and (lse[2] == 1024).all()
+
+
 def test_large_scores_and_one_token_over_many(cuda_device):
     # a page of large weights in front of many small ones, which halves hold only as multiples of 2^-24
     q, k, v, table, n = make([60000, 600], 1, 2, 64, 16, F16)
