@@ -1248,6 +1248,6 @@ extern "C" int blk_paged_attention(const blk_paged_cache_t* c, const void* q, in
     p.scale = p.sign * scale;
     if (p.scale == 0.f) p.scale = 1.17549435e-38f;  // softmax(0 * S) is the uniform distribution
     p.c = p.scale * 1.4426950408889634f;
-    const cudaError_t err = blk_launch_paged_attn(p, s, c->dtype, reinterpret_cast<cudaStream_t>(cuda_stream));
+    const cudaError_t err = blk_launch_paged_attn(p, s, c->dtype, sms, reinterpret_cast<cudaStream_t>(cuda_stream));
     return err == cudaSuccess ? BLK_OK : cuda_fail(where, err);
 }

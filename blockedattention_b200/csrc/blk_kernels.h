@@ -294,7 +294,7 @@ struct BlkPagedShape {
     int64_t work_floats;
 };
 BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int64_t kv_heads, int64_t capacity, int sms);
-cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedShape& s, int dtype, cudaStream_t st);
+cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedShape& s, int dtype, int sms, cudaStream_t st);
 
 struct BlkPagedSlotsParams {
     const int *lengths, *new_tokens;

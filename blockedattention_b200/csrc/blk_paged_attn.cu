@@ -10,6 +10,8 @@
 // warps' maxima, sums and weighted values are put together; where it goes on in another block, they go to the workspace, and
 // a second kernel joins the parts of the heads that were cut (at most two parts a block, so the workspace does
 // not grow with the lengths).  No atomics: the same call gives the same bits.
+#include <algorithm>
+
 #include "blk_device.cuh"
 #include "blk_kernels.h"
 
@@ -377,9 +379,8 @@ struct Lay {
 struct Walk {
     int r, kv, part, t, n, len, ahead;
 };
-__device__ __forceinline__ int held(const BlkPagedAttnParams& p, int r) {
-    return min(max(p.lengths[r], 0), p.capacity);
-}
+__device__ __forceinline__ int clipped(const BlkPagedAttnParams& p, int len) { return min(max(len, 0), p.capacity); }
+__device__ __forceinline__ int held(const BlkPagedAttnParams& p, int r) { return clipped(p, p.lengths[r]); }
 template <int TILE>
 __device__ __forceinline__ int tiles_of(int len) { return max(1, (int)(((unsigned)len + TILE - 1) / TILE)); }  // (an empty request's result is written, too)
 template <int TILE>
@@ -391,9 +392,9 @@ __device__ __forceinline__ void step(Walk& w, const BlkPagedAttnParams& p) {
     if (++w.kv < p.kv_heads) return;
     w.kv = 0;
     ++w.r;
-    w.len = w.ahead;
+    w.len = clipped(p, w.ahead);
     w.n = tiles_of<TILE>(w.len);
-    w.ahead = w.r + 1 < p.requests ? held(p, w.r + 1) : 0;
+    if (w.r + 1 < p.requests) w.ahead = p.lengths[w.r + 1];  // (as it is: to clip it now would wait for it)
 }
 
 template <typename Tag> struct Out;
@@ -440,9 +441,13 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     }
     blk_grid_wait();
 
-    // The lengths, added up: a run of requests for every thread.
-    Walk cw;
-    int64_t lo, hi, all = 0, blocks;
+    // The lengths, added up: a run of requests for every thread.  A range is cut by cost: to change heads costs three quarters of a tile.  Tile t of
+    // a head begins at cost 0 for t = 0, else HEAD + TIME t, and belongs to the block whose range this lies in.  With less than
+    // a head of one tile for every block tiles alone count, so that none is empty.
+    Walk cw{};
+    int64_t all, blocks, first;  // cost of everything; blocks that have a part of it; this one's first tile
+    int64_t count;
+    int TIME = 4, HEAD = 3;
     {
         const int per = (p.requests + THREADS - 1) / THREADS, r0 = min(tid * per, p.requests), r1 = min(r0 + per, p.requests);
         int64_t mine = 0;
@@ -455,45 +460,67 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         }
         if (lane == 31) sched[warp] = before;
         __syncthreads();
+        int64_t tiles = 0;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             if (w < warp) before += sched[w];
-            all += sched[w];
+            tiles += sched[w];
         }
         before -= mine;
-        all *= p.units;
-        blocks = min((int64_t)gridDim.x, all);
+        blocks = gridDim.x;
+        if (p.units * (TIME * tiles + HEAD * (int64_t)p.requests) < blocks * (TIME + HEAD)) {
+            TIME = 1;
+            HEAD = 0;
+            blocks = min(blocks, p.units * tiles);
+        }
         if (blockIdx.x >= blocks) {
             if (tid == 0) p.parts[blockIdx.x] = make_int4(0, 0, 0, 0);
             return;
         }
-        lo = quotient(blockIdx.x * all, blocks);
-        hi = quotient((blockIdx.x + 1) * all, blocks);
-        const int64_t x = quotient(lo, p.units);
-        if (x >= before && x < before + mine) {
-            int r = r0;
-            int64_t at = before;
-            int len = held(p, r), n = tiles_of<TILE>(len);
-            while (x >= at + n) {
-                at += n;
-                len = held(p, ++r);
+        all = p.units * (TIME * tiles + HEAD * (int64_t)p.requests);
+        // the two ends of the range, by the thread that has the request which each lies in
+        const int64_t lo_cost = p.units * (TIME * before + HEAD * (int64_t)r0), hi_cost = lo_cost + p.units * (TIME * mine + HEAD * (int64_t)(r1 - r0));
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e) {
+            const int64_t x = quotient((blockIdx.x + e) * all, blocks);
+            if (x < lo_cost || x >= hi_cost) continue;
+            int64_t at = lo_cost, tile = before;
+            int r = r0, len, n;
+            for (;; ++r) {
+                len = held(p, r);
                 n = tiles_of<TILE>(len);
+                const int64_t end = at + p.units * ((int64_t)TIME * n + HEAD);
+                if (x < end) break;
+                at = end;
+                tile += n;
             }
-            sched[4] = r;
-            sched[5] = lo - at * p.units;
-            sched[6] = len;
+            const int64_t span = (int64_t)TIME * n + HEAD, unit = quotient(x - at, span);
+            const int y = (int)(x - at - unit * span), t = y == 0 ? 0 : max(1, (y - HEAD + TIME - 1) / TIME);  // t = n: the next head's first
+            sched[8 + 4 * e] = p.units * tile + unit * n + t;
+            if (e == 0) {
+                sched[9] = r;
+                sched[10] = len;
+                sched[11] = unit;
+                sched[13] = t;
+            }
         }
+        if (tid == 0 && blockIdx.x + 1 == blocks) sched[12] = p.units * tiles;
         __syncthreads();
-        cw.r = (int)sched[4];
-        cw.ahead = cw.r + 1 < p.requests ? held(p, cw.r + 1) : 0;
-        cw.len = (int)sched[6];
+        first = sched[8];
+        count = sched[12] - first;
+        cw.r = (int)sched[9];
+        if (cw.r + 1 < p.requests) cw.ahead = p.lengths[cw.r + 1];
+        cw.len = (int)sched[10];
         cw.n = tiles_of<TILE>(cw.len);
-        const int unit = (int)quotient(sched[5], cw.n);
-        cw.t = (int)(sched[5] - (int64_t)unit * cw.n);
-        cw.kv = unit / p.q_units;
+        const int unit = (int)sched[11];
+        cw.kv = p.q_units == 1 ? unit : unit / p.q_units;
         cw.part = unit - cw.kv * p.q_units;
+        cw.t = (int)sched[13];
+        if (cw.t == cw.n) {
+            cw.t -= 1;
+            step<TILE>(cw, p);
+        }
     }
-    const int64_t count = hi - lo;
 
     // Copies.  A lane looks up the page of one of the warp's tokens, two tiles before its rows are asked for; eight lanes take 128
     // bytes of a row.
@@ -583,9 +610,9 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         if (ends || !more) {
             if (more) math.fetch(p, q_at(cw), rows_at(cw), lane);
             const bool begins = i >= now.t;
-            const int first = now.part * p.rows_unit, rows = rows_at(now);
+            const int rows = rows_at(now);
             float* const ws = p.work + (2 * (int64_t)blockIdx.x + (begins ? 1 : 0)) * (GU * DP + 2 * GU);
-            const int64_t head0 = (int64_t)now.r * p.heads + now.kv * p.group + first;
+            const int64_t head0 = (int64_t)now.r * p.heads + now.kv * p.group + now.part * p.rows_unit;
 #pragma unroll 1
             for (int n = 0; n < M::NT; ++n) {
                 __syncthreads();  // (what was put here before is read)
@@ -626,7 +653,8 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
                 }
             }
             if (begins && !ends) {  // the head goes on in the blocks up to the one that has its last tile
-                const int64_t last = lo + i - now.t + now.n - 1;
+                const int64_t tile = first + i - now.t, head = (int64_t)now.r * p.units + now.kv * p.q_units + now.part;  // its first tile; heads before it
+                const int64_t last = TIME * (tile + now.n - 1) + HEAD * (head + 1);  // (of two tiles or more)
                 part = make_int4((int)quotient((last + 1) * blocks - 1, all) - (int)blockIdx.x + 1, now.r, now.kv, now.part);
             }
             if (more) math.begin(extra);
@@ -636,61 +664,130 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     if (tid == 0) p.parts[blockIdx.x] = part;
 }
 
-// Joins the parts of the heads that were cut: block (c, y) those of the head that begins in block c and goes on, four query rows
-// each, four warps to a row.
+// Joins the parts of the heads that were cut.  Every block finds these heads for itself, then takes rows of them in turn: a part for
+// every warp, its statistics and values asked for together, then the warps' results as parts again.
+constexpr int JOIN_WARPS = 8, MAX_BLOCKS = 1024;
 template <typename Tag, int DP>
-__global__ void __launch_bounds__(512) blk_paged_join_kernel(const BlkPagedAttnParams p, int GU, float out_scale) {
-    __shared__ float sums[16][DP];
-    __shared__ float denom[16];
+__global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const BlkPagedAttnParams p, int GU, int blocks, float out_scale) {
+    constexpr int V = DP / 32 < 4 ? DP / 32 : 4, W = DP / 32 / V;  // vectors of V floats, W of them for a lane
+    __shared__ __align__(16) float values[JOIN_WARPS][DP];
+    __shared__ float tops[JOIN_WARPS], sums[JOIN_WARPS];
+    __shared__ uint32_t cut[MAX_BLOCKS / 32];
+    __shared__ int4 heads[MAX_BLOCKS];  // of those that were cut: parts, request, key head, part of its rows
+    __shared__ int begins[MAX_BLOCKS];  // the block that each begins in
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     blk_grid_wait();
-    const int4 part = p.parts[blockIdx.x];
-    const int n = part.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, sub = warp / 4, row = blockIdx.y * 4 + warp % 4;
-    if (n == 0) return;
-    const int kv = part.z, first = part.w * p.rows_unit, rows = min(p.rows_unit, p.group - first);
-    if ((int)blockIdx.y * 4 >= rows) return;
-    const bool mine = row < rows;
-    const int64_t size = GU * DP + 2 * GU;
-    const float* const base = p.work + 2 * (int64_t)blockIdx.x * size;  // part i > 0 is the first of block c + i
-    auto at = [&](int i) { return base + (2 * (int64_t)i + (i == 0)) * size; };
-    float top = -INFINITY;
-    if (mine)
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, at(i)[GU * DP + row]);
+    constexpr int AT_ONCE = 2;
+    int total = 0;
+    for (int base = 0; base < blocks; base += JOIN_WARPS * 32 * AT_ONCE) {
+        int4 part[AT_ONCE];
 #pragma unroll
-    for (int x = 1; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float acc[DP / 32], sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < DP / 32; ++j) acc[j] = 0.f;
-    if (mine) {
-#pragma unroll 4
-        for (int i = sub; i < n; i += 4) {
-            const float* a = at(i);
-            const float l = a[GU * DP + GU + row], w = part_weight(a[GU * DP + row], top, p.c);
-            const bool counts = part_counts(l, top);
-            if (counts) sum = fmaf(w, l, sum);
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j)
-                if (counts && lane + 32 * j < p.d) acc[j] = fmaf(w, a[row * DP + lane + 32 * j], acc[j]);
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int c = base + j * (JOIN_WARPS * 32) + tid;
+            part[j] = c < blocks ? p.parts[c] : make_int4(0, 0, 0, 0);
         }
-    }
 #pragma unroll
-    for (int j = 0; j < DP / 32; ++j) sums[warp][lane + 32 * j] = acc[j];
-    if (lane == 0) denom[warp] = sum;
-    __syncthreads();
-    const int r = warp % 4, col = lane * 4 + (warp / 4) * 128;  // (the first eight warps: 256 columns of a row)
-    if (!mine || col >= p.d || col >= DP) return;
-    const float l = denom[r] + denom[4 + r] + denom[8 + r] + denom[12 + r];
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const uint32_t word = __ballot_sync(0xffffffffu, part[j].x != 0);
+            if (lane == 0) cut[j * JOIN_WARPS + warp] = word;
+        }
+        __syncthreads();
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const float4 y = *reinterpret_cast<const float4*>(&sums[4 * s + r][col]);
-        v.x += y.x;
-        v.y += y.y;
-        v.z += y.z;
-        v.w += y.w;
+        for (int j = 0; j < AT_ONCE; ++j) {
+            int rank = total;
+            for (int w = 0; w < j * JOIN_WARPS + warp; ++w) rank += __popc(cut[w]);
+            rank += __popc(cut[j * JOIN_WARPS + warp] & ((1u << lane) - 1));
+            if (part[j].x) {
+                heads[rank] = part[j];
+                begins[rank] = base + j * (JOIN_WARPS * 32) + tid;
+            }
+        }
+        for (int w = 0; w < AT_ONCE * JOIN_WARPS; ++w) total += __popc(cut[w]);
+        __syncthreads();
     }
-    const int64_t head = (int64_t)part.y * p.heads + (int64_t)kv * p.group + first + row;
-    Out<Tag>::put4(p.out, head * p.d + col, divided(v, l, out_scale));
-    if (p.lse && col == 0) p.lse[head] = row_log(top, l, p.scale);
+    const int64_t size = GU * DP + 2 * GU;
+    for (int item = blockIdx.x; item < total * p.rows_unit; item += gridDim.x) {
+        const int which = item / p.rows_unit, row = item - which * p.rows_unit;
+        const int4 head = heads[which];
+        const int rows = min(p.rows_unit, p.group - head.w * p.rows_unit);
+        if (row >= rows) continue;
+        const float* const base = p.work + 2 * (int64_t)begins[which] * size;  // part i > 0 is the first of block c + i
+        float top = -INFINITY, sum = 0.f, acc[W][V];
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[j][e] = 0.f;
+        auto add = [&](float m, float l, const float (&y)[W][V]) {
+            const float up = fmaxf(top, m);
+            if (!part_counts(l, up)) return;  // (the same for the whole warp)
+            const bool before = part_counts(sum, up);
+            const float old = part_weight(top, up, p.c), w = part_weight(m, up, p.c);
+            sum = before ? fmaf(sum, old, w * l) : w * l;
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[j][e] = before ? fmaf(acc[j][e], old, w * y[j][e]) : w * y[j][e];
+            top = up;
+        };
+        constexpr int N = 4;
+        for (int i = warp; i < head.x; i += JOIN_WARPS * N) {
+            float m[N], l[N], y[N][W][V];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int k = i + j * JOIN_WARPS;
+                const float* at = base + (2 * (int64_t)k + (k == 0)) * size;
+                m[j] = -INFINITY;
+                l[j] = 0.f;
+                if (k >= head.x) continue;
+                m[j] = at[GU * DP + row];
+                l[j] = at[GU * DP + GU + row];
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const int col = (w * 32 + lane) * V;
+                    const float* from = at + row * DP + col;
+                    if (V == 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(from);
+                        y[j][w][0] = x.x, y[j][w][1] = x.y, y[j][w][2 % V] = x.z, y[j][w][3 % V] = x.w;
+                    } else {
+                        const float2 x = *reinterpret_cast<const float2*>(from);
+                        y[j][w][0] = x.x, y[j][w][1] = x.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) add(m[j], l[j], y[j]);
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int e = 0; e < V; ++e) values[warp][(w * 32 + lane) * V + e] = acc[w][e];
+        if (lane == 0) {
+            tops[warp] = top;
+            sums[warp] = sum;
+        }
+        __syncthreads();
+        if (tid * 4 < p.d) {
+            float t = -INFINITY, l = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < JOIN_WARPS; ++w) t = fmaxf(t, tops[w]);
+#pragma unroll
+            for (int w = 0; w < JOIN_WARPS; ++w)
+                if (part_counts(sums[w], t)) {
+                    const float f = part_weight(tops[w], t, p.c);
+                    const float4 y = *reinterpret_cast<const float4*>(&values[w][tid * 4]);
+                    l = fmaf(f, sums[w], l);
+                    v.x = fmaf(f, y.x, v.x);
+                    v.y = fmaf(f, y.y, v.y);
+                    v.z = fmaf(f, y.z, v.z);
+                    v.w = fmaf(f, y.w, v.w);
+                }
+            const int64_t at = (int64_t)head.y * p.heads + head.z * p.group + head.w * p.rows_unit + row;
+            Out<Tag>::put4(p.out, at * p.d + tid * 4, divided(v, l, out_scale));
+            if (p.lse && tid == 0) p.lse[at] = row_log(t, l, p.scale);
+        }
+        __syncthreads();
+    }
 }
 
 // The kernels: padded head dimension, query rows of a unit in eights, stages, blocks on an SM.
@@ -744,14 +841,14 @@ BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int
         tile = Lay<M>::TILE;
         ctas = M::CTAS;
     });
-    const int64_t tiles = capacity > 0 ? (capacity + tile - 1) / tile : 1, room = (int64_t)ctas * sms;
+    const int64_t tiles = capacity > 0 ? (capacity + tile - 1) / tile : 1, room = std::min(ctas * sms, MAX_BLOCKS);
     const int64_t units = requests * kv_heads * s.q_units;
     s.blocks = (int)(units >= room || tiles >= room || units * tiles >= room ? room : units * tiles);
     s.work_floats = (int64_t)s.blocks * 2 * (8 * s.NT) * (s.DP + 2);
     return s;
 }
 
-cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedShape& s, int dtype, cudaStream_t st) {
+cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedShape& s, int dtype, int sms, cudaStream_t st) {
     const int GU = 8 * s.NT;
     return with_kernel(dtype, s.DP, s.NT, [&](auto m) {
         typedef typename decltype(m)::T M;
@@ -760,7 +857,8 @@ cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedSha
         if (e != cudaSuccess) return e;
         e = blk_launch(true, kern, dim3((unsigned)s.blocks), dim3(THREADS), (size_t)Lay<M>::BYTES, st, p);
         if (e != cudaSuccess || s.blocks == 1) return e;
-        return blk_launch(true, blk_paged_join_kernel<typename M::Tag, M::DP>, dim3((unsigned)s.blocks, (unsigned)(s.rows_unit + 3) / 4), dim3(512),
-                          (size_t)0, st, p, GU, M::OUT_SCALE);
+        const int items = (s.blocks - 1) * s.rows_unit, most = 4 * sms;
+        return blk_launch(true, blk_paged_join_kernel<typename M::Tag, M::DP>, dim3((unsigned)(items < most ? items : most)), dim3(JOIN_WARPS * 32),
+                          (size_t)0, st, p, GU, s.blocks, M::OUT_SCALE);
     });
 }
