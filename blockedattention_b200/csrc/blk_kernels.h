@@ -284,6 +284,7 @@ struct BlkPagedAttnParams {
     float* lse;
     float* work;
     int4* parts;
+    int one_page;          // filled by the launcher: a warp's tokens of a tile never lie on two pages
     float c, scale;        // |scale| log2(e), |scale|
     float sign;            // of the scale
 };

@@ -36,11 +36,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float4 lds128(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-    return v;
-}
 // A part of a row: maximum m and sum l of its weights relative to m.  l = 0: it saw no token, and its values are not there.
 // l = inf, m = -inf: it saw scores of -inf alone, which count only where every part is like that (0 / 0).  A NaN in l is kept.
 __device__ __forceinline__ bool part_counts(float l, float top) { return l != 0.f && !(l == INFINITY && top > -INFINITY); }
@@ -78,10 +73,11 @@ template <> struct PSplit<BlkHalfTag> {
     }
 };
 
-template <typename Tag_, int DP_, int NT_, int STAGES_, int CTAS_>
+template <typename Tag_, int DP_, int NT_, int STAGES_, int CTAS_, int PASS_>
 struct Math16 {
     typedef Tag_ Tag;
-    static constexpr int DP = DP_, NT = NT_, GU = 8 * NT, E = 2, TW = 16, STAGES = STAGES_, CTAS = CTAS_, RB = DP * E, EXTRA = 0;
+    static constexpr int DP = DP_, NT = NT_, GU = 8 * NT, E = 2, TW = 16, STAGES = STAGES_, CTAS = CTAS_, EXTRA = 0,
+                         PASS = PASS_;  // rows put together at a time
     uint32_t qf[DP / 16][NT][2];
     float o[DP / 16][NT][4];
     float m[NT][2], l[NT][2];
@@ -127,11 +123,11 @@ struct Math16 {
                 for (int e = 0; e < 4; ++e) part[i][n][e] = 0.f;
         {
             const int row = lane & 15;
-            const uint32_t base = sK + row * RB, x = ((lane >> 4) ^ (row & 7)) << 4;
+            const uint32_t base = sK + row * 128, x = ((lane >> 4) ^ (row & 7)) << 4;
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
                 uint32_t a[4];
-                blk_ldmatrix_x4(a, base + ((kk * 32) ^ x));
+                blk_ldmatrix_x4(a, base + kk / 4 * (TW * 128) + ((kk % 4 * 32) ^ x));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) blk_mma16816<Tag>(part[kk % CHAINS][n], a[0], a[1], a[2], a[3], qf[kk][n][0], qf[kk][n][1]);
             }
@@ -184,11 +180,11 @@ struct Math16 {
             for (int e = 0; e < 2; ++e) l[n][e] += s[n][e] + s[n][2 + e];
         {
             const int row = (lane & 7) + ((lane >> 4) << 3);
-            const uint32_t base = sV + row * RB, x = (((lane >> 3) & 1) ^ (row & 7)) << 4;
+            const uint32_t base = sV + row * 128, x = (((lane >> 3) & 1) ^ (row & 7)) << 4;
 #pragma unroll
             for (int mm = 0; mm < DP / 16; ++mm) {
                 uint32_t a[4];
-                blk_ldmatrix_x4_trans(a, base + ((mm * 32) ^ x));
+                blk_ldmatrix_x4_trans(a, base + mm / 4 * (TW * 128) + ((mm % 4 * 32) ^ x));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     blk_mma16816<Tag>(o[mm][n], a[0], a[1], a[2], a[3], hi[n][0], hi[n][1]);
@@ -214,148 +210,201 @@ struct Math16 {
                 }
             }
     }
-    // this warp's values of query rows 8n .. 8n+7, relative to its own maxima; rows: how many of all rows there are
-    __device__ __forceinline__ void put(int n_, float* dst, int rows, int lane) {
-        const int q = (lane & 3) * 2;
+    // this warp's values of query rows PASS n .. , relative to its own maxima; rows: how many of all rows there are
+    __device__ __forceinline__ void put(int pass, float* dst, int rows, int lane) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (n == n_ && n * 8 + q < rows) {
+        for (int n = 0; n < NT; ++n) {
+            const int row = n * 8 + (lane & 3) * 2, q = row - pass * PASS;
+            if (q < 0 || q >= PASS || row >= rows) continue;
 #pragma unroll
-                for (int mm = 0; mm < DP / 16; ++mm) {
-                    const int col = mm * 16 + lane / 4;
-                    dst[merge_at<DP>(q, col)] = o[mm][n][0];
-                    dst[merge_at<DP>(q + 1, col)] = o[mm][n][1];
-                    dst[merge_at<DP>(q, col + 8)] = o[mm][n][2];
-                    dst[merge_at<DP>(q + 1, col + 8)] = o[mm][n][3];
-                }
+            for (int mm = 0; mm < DP / 16; ++mm) {
+                const int col = mm * 16 + lane / 4;
+                dst[merge_at<DP>(q, col)] = o[mm][n][0];
+                dst[merge_at<DP>(q + 1, col)] = o[mm][n][1];
+                dst[merge_at<DP>(q, col + 8)] = o[mm][n][2];
+                dst[merge_at<DP>(q + 1, col + 8)] = o[mm][n][3];
             }
+        }
     }
     static constexpr float OUT_SCALE = 1.f / PSplit<Tag>::SCALE;
 };
 
 // ---- the same in 32 bits -------------------------------------------------------------------------------
-// A lane holds one token (part of its row: 32 / TW lanes share one) for the scores and DP / 32 columns for the values; q and the
-// weights are broadcast from shared memory.
+// A lane holds four columns (eight at 256) of q, of every token's key and value and of the result, two operations to an instruction; below 128
+// columns half a warp does, and the warp takes two tokens at once.  A token's eight scores (a sum over the lanes each) are
+// added by halves, so that 32 sums of four tokens cost 31 exchanges and end up one in each lane, where the softmax goes on.
 struct BlkFloatTag {};
-template <int DP_, int TW_, int STAGES_, int CTAS_>
+template <int DP_, int TW_, int STAGES_, int CTAS_, int PASS_>
 struct Math32 {
     typedef BlkFloatTag Tag;
-    static constexpr int DP = DP_, NT = 1, GU = 8, E = 4, TW = TW_, STAGES = STAGES_, CTAS = CTAS_, RB = DP * E, PARTS = 32 / TW, W = DP / 32;
-    static constexpr int EXTRA = 8 * DP * 4 + WARPS * TW * 8 * 4;  // q, weights of every warp
-    float o[8][W];
-    float m[8], l[8];
+    static constexpr int DP = DP_, GU = 8, E = 4, TW = TW_, STAGES = STAGES_, CTAS = CTAS_, PASS = PASS_;
+    static constexpr int LANES = DP == 64 ? 16 : 32, C = DP / 4 / LANES, PAR = 32 / LANES, BATCHES = TW / 4;  // lanes of a token, its vectors in a lane, tokens at once
+    static constexpr int EXTRA = WARPS * TW * 8 * 4;  // every warp's weights
+    float2 q[8][C][2], o[8][C][2];
+    float m, l;  // of this lane's row
     bool seen;
+    int d;
 
-    float qv[8 * DP / THREADS];
-    __device__ __forceinline__ void fetch(const BlkPagedAttnParams& p, const char* q, int rows, int) {
+    static __device__ __forceinline__ int row_of(int lane) { return PAR == 2 ? lane >> 1 & 7 : lane >> 2; }
+    static __device__ __forceinline__ int token_of(int lane) { return PAR == 2 ? (lane & 1) * 2 + (lane >> 4) : lane & 3; }
+    static __device__ __forceinline__ int col_of(int c, int lane) { return (c * LANES + lane % LANES) * 4; }
+
+    __device__ __forceinline__ void fetch(const BlkPagedAttnParams& p, const char* at, int rows, int lane) {
+        d = p.d;
 #pragma unroll
-        for (int j = 0; j < 8 * DP / THREADS; ++j) {
-            const int i = j * THREADS + threadIdx.x, row = i / DP, col = i % DP;
-            qv[j] = row < rows && col < p.d ? reinterpret_cast<const float*>(q + row * p.q_head_stride)[col] : 0.f;
-        }
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < rows && col_of(c, lane) < p.d) v = *reinterpret_cast<const float4*>(at + i * p.q_head_stride + col_of(c, lane) * 4);
+                q[i][c][0] = make_float2(v.x, v.y);
+                q[i][c][1] = make_float2(v.z, v.w);
+            }
     }
-    // (behind a barrier that no warp reaches before its last tile of the head before)
-    __device__ __forceinline__ void begin(uint32_t sx) {
+    __device__ __forceinline__ void begin(uint32_t) {
 #pragma unroll
-        for (int j = 0; j < 8 * DP / THREADS; ++j) blk_sts_f32(sx + (j * THREADS + threadIdx.x) * 4, qv[j]);
-        __syncthreads();
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.f;
-#pragma unroll
-            for (int j = 0; j < W; ++j) o[i][j] = 0.f;
-        }
+            for (int c = 0; c < C; ++c) o[i][c][0] = o[i][c][1] = make_float2(0.f, 0.f);
+        m = -INFINITY;
+        l = 0.f;
         seen = false;
     }
-
-    __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float sign, float c, uint32_t sx, int lane) {
-        seen = true;
-        const int tok = lane % TW, part = lane / TW;
-        const bool valid = mask >> tok & 1;
-        float s[8];
+    // four floats of token t, vector c
+    static __device__ __forceinline__ float4 vec(uint32_t s, int t, int c, int lane) {
+        const int x = c * LANES + lane % LANES;
+        float4 v;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                     : "r"(s + x / 8 * (TW * 128) + t * 128 + (((x & 7) ^ (t & 7)) << 4)));
+        return v;
+    }
+    // a[0 .. 2N) of this lane and of the one that differs in bit x: the sums of the half that the bit chooses
+    template <int N>
+    static __device__ __forceinline__ void halve(const float* a, float* b, int x, int lane) {
+        const bool high = lane & x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = 0.f;
-#pragma unroll 4
-        for (int j = 0; j < DP / 4 / PARTS; ++j) {
-            const int ch = j * PARTS + part;
-            const float4 k = lds128(sK + tok * RB + ((ch ^ (tok & 7)) << 4));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 q = lds128(sx + (i * DP + ch * 4) * 4);
-                s[i] = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, s[i]))));
-            }
+        for (int i = 0; i < N; ++i) {
+            const float keep = high ? a[i + N] : a[i], give = high ? a[i] : a[i + N];
+            b[i] = keep + __shfl_xor_sync(0xffffffffu, give, x);
         }
-        const uint32_t sp = sx + 8 * DP * 4 + (threadIdx.x / 32) * (TW * 8 * 4);
+    }
+
+    __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float sign, float scale, uint32_t sx, int lane) {
+        constexpr int TOP = PAR == 2 ? 8 : 16;
+        seen = true;
+        const int row = row_of(lane), tok = token_of(lane);
+        float s[BATCHES];
+#pragma unroll
+        for (int b = 0; b < BATCHES; ++b) {
+            float r[4 / PAR];
+#pragma unroll
+            for (int j = 0; j < 4 / PAR; ++j) {
+                const int t = 4 * b + (PAR == 2 ? 2 * j + (lane >> 4) : j);
+                float a[8], h4[4], h2[2];
+                float4 k[C];
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    k[c] = vec(sK, t, c, lane);
+                    if (col_of(c, lane) >= d) k[c] = make_float4(0.f, 0.f, 0.f, 0.f);  // (no copy has written there)
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float2 x = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        x = blk_fma2(make_float2(k[c].x, k[c].y), q[i][c][0], x);
+                        x = blk_fma2(make_float2(k[c].z, k[c].w), q[i][c][1], x);
+                    }
+                    a[i] = x.x + x.y;
+                }
+                halve<4>(a, h4, TOP, lane);
+                halve<2>(h4, h2, TOP / 2, lane);
+                halve<1>(h2, r + j, TOP / 4, lane);
+            }
+            if (PAR == 1) {
+                float h[2];
+                halve<2>(r, h, 2, lane);
+                halve<1>(h, s + b, 1, lane);
+            } else {
+                halve<1>(r, s + b, 1, lane);
+            }
+            s[b] *= sign;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < BATCHES; ++b)
+            if (mask >> (4 * b + tok) & 1) top = fmaxf(top, s[b]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, PAR == 2 ? 16 : 2));
+        top = fmaxf(top, m);
+        const float ref = top == -INFINITY ? 0.f : top, alpha = blk_exp2((m - ref) * scale);
+        const bool grew = __any_sync(0xffffffffu, top > m);
+        m = top;
+        const uint32_t sp = sx + (threadIdx.x / 32) * (TW * 8 * 4);
+        if (grew) l *= alpha;
         __syncwarp();  // (the weights of the tile before are read)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int b = 0; b < BATCHES; ++b) {
+            const float w = mask >> (4 * b + tok) & 1 ? blk_exp2((s[b] - ref) * scale) : 0.f;
+            l += w;
+            blk_sts_f32(sp + ((4 * b + tok) * 8 + row) * 4, w);
+        }
+        if (grew) {
 #pragma unroll
-            for (int x = TW; x < 32; x *= 2) s[i] += __shfl_xor_sync(0xffffffffu, s[i], x);
-            s[i] *= sign;
-            float t = valid ? s[i] : -INFINITY;
+            for (int i = 0; i < 8; ++i) {
+                const float x = __shfl_sync(0xffffffffu, alpha, i * (PAR == 2 ? 2 : 4));
 #pragma unroll
-            for (int x = 1; x < TW; x *= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-            const float top = fmaxf(m[i], t), ref = top == -INFINITY ? 0.f : top;
-            if (top > m[i]) {  // (the same for the whole warp)
-                const float alpha = blk_exp2((m[i] - ref) * c);
-                l[i] *= alpha;
+                for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int j = 0; j < W; ++j) o[i][j] *= alpha;
-            }
-            m[i] = top;
-            s[i] = valid ? blk_exp2((s[i] - ref) * c) : 0.f;
-            if (part == 0) {
-                l[i] += s[i];
-                blk_sts_f32(sp + (tok * 8 + i) * 4, s[i]);
+                    for (int e = 0; e < 2; ++e) o[i][c][e] = blk_mul2(o[i][c][e], make_float2(x, x));
             }
         }
         __syncwarp();
 #pragma unroll 4
-        for (int t = 0; t < TW; ++t) {
-            const float4 a = lds128(sp + t * 32), b = lds128(sp + t * 32 + 16);
-            const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            float v[W];
-            if (W == 2) {
-                const uint32_t at = sV + t * RB + (((lane >> 1) ^ (t & 7)) << 4) + (lane & 1) * 8;
-                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];\n" : "=f"(v[0]), "=f"(v[1]) : "r"(at));
-            } else {
+        for (int u = 0; u < TW / PAR; ++u) {
+            const int t = PAR == 2 ? 2 * u + (lane >> 4) : u;
+            float w[8];
 #pragma unroll
-                for (int j = 0; j < W / 4; ++j) {
-                    const float4 x = lds128(sV + t * RB + (((lane + 32 * j) ^ (t & 7)) << 4));
-                    v[(4 * j) % W] = x.x;
-                    v[(4 * j + 1) % W] = x.y;
-                    v[(4 * j + 2) % W] = x.z;
-                    v[(4 * j + 3) % W] = x.w;
+            for (int i = 0; i < 2; ++i)
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                             : "=f"(w[4 * i]), "=f"(w[4 * i + 1]), "=f"(w[4 * i + 2]), "=f"(w[4 * i + 3])
+                             : "r"(sp + t * 32 + i * 16));
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float4 v = vec(sV, t, c, lane);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    o[i][c][0] = blk_fma2(make_float2(w[i], w[i]), make_float2(v.x, v.y), o[i][c][0]);
+                    o[i][c][1] = blk_fma2(make_float2(w[i], w[i]), make_float2(v.z, v.w), o[i][c][1]);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int j = 0; j < W; ++j) o[i][j] = fmaf(w[i], v[j], o[i][j]);
         }
     }
 
     __device__ __forceinline__ void stats(float* sm, float* sl, int lane) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float t = l[i];
-#pragma unroll
-            for (int x = 1; x < TW; x *= 2) t += __shfl_xor_sync(0xffffffffu, t, x);
-            if (lane == 0) {
-                sm[i] = m[i];
-                sl[i] = seen && t == 0.f ? INFINITY : t;
-            }
+        float t = l;
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, PAR == 2 ? 16 : 2);
+        if (token_of(lane) == 0) {
+            sm[row_of(lane)] = m;
+            sl[row_of(lane)] = seen && t == 0.f ? INFINITY : t;
         }
     }
-    __device__ __forceinline__ void put(int, float* dst, int rows, int lane) {
+    __device__ __forceinline__ void put(int n, float* dst, int rows, int lane) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < rows) {
+            if (i / PASS == n && i < rows) {
 #pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    const int col = W == 2 ? lane * 2 + j : (j / 4) * 128 + lane * 4 + (j & 3);
-                    dst[merge_at<DP>(i, col)] = o[i][j];
+                for (int c = 0; c < C; ++c) {
+                    float4 v = make_float4(o[i][c][0].x, o[i][c][0].y, o[i][c][1].x, o[i][c][1].y);
+                    if (PAR == 2) {
+                        v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+                        v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+                        v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
+                        v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+                    }
+                    if (PAR == 1 || lane < 16) *reinterpret_cast<float4*>(dst + merge_at<DP>(i % PASS, col_of(c, lane))) = v;
                 }
             }
     }
@@ -363,13 +412,14 @@ struct Math32 {
 };
 
 // ---- shared memory -------------------------------------------------------------------------------------
+// A warp's stage: the keys of its TW tokens, then the values, each as halves of 128 bytes of all rows, 16-byte pieces swizzled by the row.
 template <typename M>
 struct Lay {
-    static constexpr int TILE = WARPS * M::TW;
-    static constexpr int HALF = M::TW * M::RB;                       // a warp's keys, or values, of a stage
-    static constexpr int RING = WARPS * M::STAGES * 2 * HALF;
-    static constexpr int MERGE = WARPS * 8 * M::DP * 4;
-    static constexpr int STATS = 2 * WARPS * M::GU * 4;              // maxima and sums of the warps
+    static constexpr int TILE = WARPS * M::TW, HALVES = (M::DP * M::E + 127) / 128;
+    static constexpr int SIDE = HALVES * M::TW * 128;
+    static constexpr int RING = WARPS * M::STAGES * 2 * SIDE;
+    static constexpr int MERGE = WARPS * M::PASS * M::DP * 4;
+    static constexpr int STATS = 2 * WARPS * M::GU * 4;  // maxima and sums of the warps
     static constexpr int MASKS = WARPS * M::STAGES * 4;
     static constexpr int BYTES = RING + MERGE + M::EXTRA + STATS + MASKS;
     static_assert((BYTES + 1024) * M::CTAS <= 228 * 1024, "the blocks that a kernel is made for fit on an SM");
@@ -424,7 +474,7 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (a | 
 template <typename M>
 __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const BlkPagedAttnParams p) {
     typedef Lay<M> L;
-    constexpr int DP = M::DP, GU = M::GU, TW = M::TW, RB = M::RB, STAGES = M::STAGES, TILE = L::TILE, CPR = RB / 16;
+    constexpr int DP = M::DP, GU = M::GU, TW = M::TW, STAGES = M::STAGES, TILE = L::TILE, HALVES = L::HALVES, PASS = M::PASS;
     extern __shared__ __align__(128) uint8_t smem[];
     float* const merge = reinterpret_cast<float*>(smem + L::RING);
     float* const sm_m = reinterpret_cast<float*>(smem + L::RING + L::MERGE + M::EXTRA);
@@ -432,10 +482,10 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     uint32_t* const masks = reinterpret_cast<uint32_t*>(sm_l + WARPS * GU) + threadIdx.x / 32 * STAGES;
     int64_t* const sched = reinterpret_cast<int64_t*>(merge);  // (up to the first merge)
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    const uint32_t ring = blk_smem_u32(smem) + warp * (STAGES * 2 * L::HALF), extra = blk_smem_u32(smem) + L::RING + L::MERGE;
+    const uint32_t ring = blk_smem_u32(smem) + warp * (STAGES * 2 * L::SIDE), extra = blk_smem_u32(smem) + L::RING + L::MERGE;
     const int chunks = p.d * M::E / 16;
-    if (chunks < CPR) {  // columns beyond d take part in the products, and no copy writes them
-        for (int i = lane; i < STAGES * 2 * L::HALF / 16; i += 32)
+    if (chunks < HALVES * 8) {  // columns beyond d take part in the products, and no copy writes them
+        for (int i = lane; i < STAGES * 2 * L::SIDE / 16; i += 32)
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(ring + i * 16), "r"(0) : "memory");
         __syncwarp();
     }
@@ -522,52 +572,90 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         }
     }
 
-    // Copies.  A lane looks up the page of one of the warp's tokens, two tiles before its rows are asked for; eight lanes take 128
-    // bytes of a row.
     M math;
     auto q_at = [&](const Walk& w) { return p.q + w.r * p.q_row_stride + (int64_t)(w.kv * p.group + w.part * p.rows_unit) * p.q_head_stride; };
     auto rows_at = [&](const Walk& w) { return min(p.rows_unit, p.group - w.part * p.rows_unit); };
     math.fetch(p, q_at(cw), rows_at(cw), lane);
+    // Copies.  Where pages are whole numbers of a warp's tokens (one_page), these lie side by side on one page; else a lane looks up the page of one
+    // of them.  That is done two tiles before the rows are asked for; eight lanes take 128 bytes of a row.
     Walk pw = cw;
-    int entry = -1, entry2 = -1;
-    int64_t inner = 0, inner2 = 0;
+    int entry = -1, soon = -1, n_here = 0, n_soon = 0;
+    int64_t inner = 0, inner_soon = 0;
     auto look = [&]() {
-        const unsigned tok = (unsigned)pw.t * TILE + warp * TW + lane;
-        entry2 = -1;
-        if (lane < TW && tok < (unsigned)pw.len) {
+        const unsigned own = p.one_page ? 0 : lane, from = (unsigned)pw.t * TILE + warp * TW, tok = from + own;
+        n_soon = min(max((int)((unsigned)pw.len - from), 0), TW);
+        soon = -1;
+        if (tok < (unsigned)pw.len && own < TW) {
             const unsigned col = (__umulhi(tok, p.page.magic) + tok) >> p.page.shift;
-            entry2 = p.table[pw.r * p.table_stride + col];
-            inner2 = (int64_t)(tok - col * p.page.d) * p.token_stride + pw.kv * p.head_stride;
+            soon = p.table[pw.r * p.table_stride + col];
+            inner_soon = (int64_t)(tok - col * p.page.d) * p.token_stride + pw.kv * p.head_stride;
         }
     };
     const int piece = lane & 7, row8 = lane >> 3;
     auto load = [&](int stage) {
         const bool there = entry >= 0 && entry < p.pages;
-        const int64_t off = there ? entry * p.page_stride + inner : -1;
-        const uint32_t mask = __ballot_sync(0xffffffffu, there);
-        if (lane == 0) masks[stage] = mask;
-        if (!mask) return;
-        const uint32_t to = ring + stage * (2 * L::HALF);
+        const uint32_t to = ring + stage * (2 * L::SIDE) + row8 * 128;
+        const uint32_t even = (piece ^ row8) << 4;  // (of rows 4 i + row8: swizzled by their number, so two places)
+        uint32_t mask;
+        if (p.one_page) {
+            mask = there ? (uint32_t)((1ull << n_here) - 1) : 0u;
+            if (mask) {
+                const int64_t off = entry * p.page_stride + inner + row8 * p.token_stride + piece * 16;
+                const char *k = p.k + off, *v = p.v + off;
+                if (n_here == TW) {
 #pragma unroll
-        for (int i = 0; i < TW / 4; ++i) {
-            const int row = i * 4 + row8;
-            const int64_t o = __shfl_sync(0xffffffffu, off, row);
-            const bool have = o >= 0;
-            const char *const k = p.k + (have ? o : 0) + piece * 16, *const v = p.v + (have ? o : 0) + piece * 16;
-            const uint32_t dst = to + row * RB + ((piece ^ (row & 7)) << 4);
+                    for (int i = 0; i < TW / 4; ++i) {
 #pragma unroll
-            for (int j = 0; j < CPR / 8; ++j)
-                if (piece + 8 * j < chunks) {
-                    if (have) cp_async16(dst + 128 * j, k + 128 * j);
-                    cp_async16_or_zeros(dst + L::HALF + 128 * j, v + 128 * j, have);  // (a weight of zero times what lies there)
+                        for (int j = 0; j < HALVES; ++j)
+                            if (piece + 8 * j < chunks) {
+                                cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), k + 128 * j);
+                                cp_async16(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), v + 128 * j);
+                            }
+                        k += 4 * p.token_stride;
+                        v += 4 * p.token_stride;
+                    }
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < TW / 4; ++i) {
+                        const bool have = i * 4 + row8 < n_here;  // (the last rows lie behind the request's end: not read)
+#pragma unroll
+                        for (int j = 0; j < HALVES; ++j)
+                            if (piece + 8 * j < chunks) {
+                                if (have) cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), k + 128 * j);
+                                cp_async16_or_zeros(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), have ? v + 128 * j : p.v, have);
+                            }
+                        k += 4 * p.token_stride;
+                        v += 4 * p.token_stride;
+                    }
                 }
+            }
+        } else {
+            const int64_t off = there ? entry * p.page_stride + inner : -1;
+            mask = __ballot_sync(0xffffffffu, there);
+            if (mask) {
+#pragma unroll 2
+                for (int i = 0; i < TW / 4; ++i) {
+                    const int64_t o = __shfl_sync(0xffffffffu, off, i * 4 + row8);
+                    const bool have = o >= 0;
+                    const int64_t at = (have ? o : 0) + piece * 16;
+#pragma unroll
+                    for (int j = 0; j < HALVES; ++j)
+                        if (piece + 8 * j < chunks) {
+                            if (have) cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), p.k + at + 128 * j);
+                            cp_async16_or_zeros(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), p.v + at + 128 * j, have);
+                        }
+                }
+            }
         }
+        // (a weight of zero must not meet what lies in a value's place: zeros are put there)
+        if (lane == 0) masks[stage] = mask;
     };
     int64_t loaded = 0;
     int into = 0;
     auto look_on = [&](int64_t i) {
-        entry = entry2;
-        inner = inner2;
+        entry = soon;
+        inner = inner_soon;
+        n_here = n_soon;
         if (i < count) {
             step<TILE>(pw, p);
             if (pw.t == 0 && warp == 0 && lane < rows_at(pw)) {  // a new head: its queries are wanted soon
@@ -600,8 +688,8 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         next();
         const uint32_t mask = masks[stage];
         if (mask) {
-            const uint32_t sK = ring + stage * (2 * L::HALF);
-            math.tile(sK, sK + L::HALF, mask, p.sign, p.c, extra, lane);
+            const uint32_t sK = ring + stage * (2 * L::SIDE);
+            math.tile(sK, sK + L::SIDE, mask, p.sign, p.c, extra, lane);
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         const bool ends = cw.t + 1 == cw.n, more = i + 1 < count;
@@ -614,14 +702,14 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
             float* const ws = p.work + (2 * (int64_t)blockIdx.x + (begins ? 1 : 0)) * (GU * DP + 2 * GU);
             const int64_t head0 = (int64_t)now.r * p.heads + now.kv * p.group + now.part * p.rows_unit;
 #pragma unroll 1
-            for (int n = 0; n < M::NT; ++n) {
+            for (int n = 0; n * PASS < rows; ++n) {
                 __syncthreads();  // (what was put here before is read)
                 if (n == 0) math.stats(sm_m + warp * GU, sm_l + warp * GU, lane);
-                if (math.seen) math.put(n, merge + warp * (8 * DP), rows, lane);
+                if (math.seen) math.put(n, merge + warp * (PASS * DP), rows, lane);
                 __syncthreads();
-                const int here = min(8, rows - n * 8);
+                const int here = min(PASS, rows - n * PASS);
                 for (int x = tid; x < here * (DP / 4); x += THREADS) {
-                    const int q = x / (DP / 4), col = x % (DP / 4) * 4, row = n * 8 + q;
+                    const int q = x / (DP / 4), col = x % (DP / 4) * 4, row = n * PASS + q;
                     if (col >= p.d) continue;
                     float top = sm_m[row], l = 0.f;
 #pragma unroll
@@ -631,7 +719,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
                     for (int w = 0; w < WARPS; ++w) {
                         const float lw = sm_l[w * GU + row], f = part_weight(sm_m[w * GU + row], top, p.c);
                         if (part_counts(lw, top)) {
-                            const float4 y = *reinterpret_cast<const float4*>(merge + w * (8 * DP) + merge_at<DP>(q, col));
+                            const float4 y = *reinterpret_cast<const float4*>(merge + w * (PASS * DP) + merge_at<DP>(q, col));
                             l = fmaf(f, lw, l);
                             v.x = fmaf(f, y.x, v.x);
                             v.y = fmaf(f, y.y, v.y);
@@ -669,7 +757,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
 constexpr int JOIN_WARPS = 8, MAX_BLOCKS = 1024;
 template <typename Tag, int DP>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const BlkPagedAttnParams p, int GU, int blocks, float out_scale) {
-    constexpr int V = DP / 32 < 4 ? DP / 32 : 4, W = DP / 32 / V;  // vectors of V floats, W of them for a lane
+    constexpr int V = DP % 128 == 0 ? 4 : DP % 64 == 0 ? 2 : 1, W = DP / 32 / V;  // vectors of V floats, W of them for a lane
     __shared__ __align__(16) float values[JOIN_WARPS][DP];
     __shared__ float tops[JOIN_WARPS], sums[JOIN_WARPS];
     __shared__ uint32_t cut[MAX_BLOCKS / 32];
@@ -747,10 +835,12 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const B
                     const float* from = at + row * DP + col;
                     if (V == 4) {
                         const float4 x = *reinterpret_cast<const float4*>(from);
-                        y[j][w][0] = x.x, y[j][w][1] = x.y, y[j][w][2 % V] = x.z, y[j][w][3 % V] = x.w;
-                    } else {
+                        y[j][w][0] = x.x, y[j][w][1 % V] = x.y, y[j][w][2 % V] = x.z, y[j][w][3 % V] = x.w;
+                    } else if (V == 2) {
                         const float2 x = *reinterpret_cast<const float2*>(from);
-                        y[j][w][0] = x.x, y[j][w][1] = x.y;
+                        y[j][w][0] = x.x, y[j][w][1 % V] = x.y;
+                    } else {
+                        y[j][w][0] = *from;
                     }
                 }
             }
@@ -790,19 +880,22 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const B
     }
 }
 
-// The kernels: padded head dimension, query rows of a unit in eights, stages, blocks on an SM.
+// The kernels: padded head dimension, query rows of a unit in eights, stages, blocks on an SM, rows put together at a time.
 template <typename Tag> struct Kernels16 {
-    typedef Math16<Tag, 64, 1, 4, 3> D64N1;
-    typedef Math16<Tag, 64, 2, 4, 3> D64N2;
-    typedef Math16<Tag, 64, 3, 4, 2> D64N3;
-    typedef Math16<Tag, 64, 4, 4, 2> D64N4;
-    typedef Math16<Tag, 128, 1, 3, 2> D128N1;
-    typedef Math16<Tag, 128, 2, 3, 2> D128N2;
-    typedef Math16<Tag, 256, 1, 3, 1> D256N1;
+    typedef Math16<Tag, 64, 1, 4, 3, 8> D64N1;
+    typedef Math16<Tag, 64, 2, 4, 3, 8> D64N2;
+    typedef Math16<Tag, 64, 3, 4, 2, 8> D64N3;
+    typedef Math16<Tag, 64, 4, 4, 2, 8> D64N4;
+    typedef Math16<Tag, 96, 1, 3, 2, 8> D96N1;
+    typedef Math16<Tag, 96, 2, 3, 2, 8> D96N2;
+    typedef Math16<Tag, 128, 1, 3, 2, 8> D128N1;
+    typedef Math16<Tag, 128, 2, 3, 2, 8> D128N2;
+    typedef Math16<Tag, 192, 1, 2, 2, 4> D192N1;
+    typedef Math16<Tag, 256, 1, 3, 1, 4> D256N1;
 };
-typedef Math32<64, 16, 3, 2> F64;
-typedef Math32<128, 16, 3, 1> F128;
-typedef Math32<256, 8, 2, 1> F256;
+typedef Math32<64, 16, 3, 2, 8> F64;
+typedef Math32<128, 8, 3, 2, 4> F128;
+typedef Math32<256, 8, 3, 1, 4> F256;
 
 // f(the kernel's type) for what a call needs
 template <typename M> struct Of { typedef M T; };
@@ -816,8 +909,9 @@ auto with_kernel(int dtype, int DP, int NT, F f) {
             if (NT == 3) return f(Of<typename K::D64N3>{});
             return f(Of<typename K::D64N4>{});
         }
+        if (DP == 96) return NT == 1 ? f(Of<typename K::D96N1>{}) : f(Of<typename K::D96N2>{});
         if (DP == 128) return NT == 1 ? f(Of<typename K::D128N1>{}) : f(Of<typename K::D128N2>{});
-        return f(Of<typename K::D256N1>{});
+        return DP == 192 ? f(Of<typename K::D192N1>{}) : f(Of<typename K::D256N1>{});
     };
     if (dtype == BLK_F16) return half(BlkHalfTag{});
     if (dtype == BLK_BF16) return half(BlkBf16Tag{});
@@ -830,8 +924,9 @@ auto with_kernel(int dtype, int DP, int NT, F f) {
 // own, which read the keys again.
 BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int64_t kv_heads, int64_t capacity, int sms) {
     BlkPagedShape s{};
-    s.DP = d <= 64 ? 64 : d <= 128 ? 128 : 256;
-    const int most = dtype == BLK_F32 ? 8 : s.DP == 64 ? 32 : s.DP == 128 ? 16 : 8;
+    if (dtype == BLK_F32) s.DP = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+    else s.DP = d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256;
+    const int most = dtype == BLK_F32 ? 8 : s.DP == 64 ? 32 : s.DP <= 128 ? 16 : 8;
     s.q_units = (group + most - 1) / most;
     s.rows_unit = (group + s.q_units - 1) / s.q_units;
     s.NT = (s.rows_unit + 7) / 8;
@@ -848,10 +943,12 @@ BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int
     return s;
 }
 
-cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p, const BlkPagedShape& s, int dtype, int sms, cudaStream_t st) {
+cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p_in, const BlkPagedShape& s, int dtype, int sms, cudaStream_t st) {
     const int GU = 8 * s.NT;
     return with_kernel(dtype, s.DP, s.NT, [&](auto m) {
         typedef typename decltype(m)::T M;
+        BlkPagedAttnParams p = p_in;
+        p.one_page = p.page.d % M::TW == 0;
         auto kern = blk_paged_attn_kernel<M>;
         cudaError_t e = blk_func_smem(reinterpret_cast<const void*>(kern), Lay<M>::BYTES);
         if (e != cudaSuccess) return e;
