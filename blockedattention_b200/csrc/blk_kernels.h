@@ -288,10 +288,9 @@ struct BlkPagedAttnParams {
     float c, scale;        // |scale| log2(e), |scale|
     float sign;            // of the scale
 };
-// How a call is cut: padded head dimension, units a key head's query rows are taken in, their rows and eights of rows,
-// blocks, and what these leave for the join.
+// How a call is cut: padded head dimension, units a key head's query rows are taken in, their rows and the kernel's, blocks, and what these leave for the join.
 struct BlkPagedShape {
-    int DP, q_units, rows_unit, NT, blocks;
+    int DP, q_units, rows_unit, GU, blocks;
     int64_t work_floats;
 };
 BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int64_t kv_heads, int64_t capacity, int sms);

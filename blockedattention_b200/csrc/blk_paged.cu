@@ -9,9 +9,9 @@ __device__ __forceinline__ unsigned divide(unsigned n, const BlkDivisor& d) { re
 // ---- slots -----------------------------------------------------------------------------------------------
 // Request r holds old_r tokens and gets new_r.  Its pages a_r = ceil(old_r / size) up to b_r = ceil((old_r + new_r) / size) are new:
 // they come from the list of free pages behind what the requests before it take.  Two prefix sums over the requests (tokens,
-// pages) therefore say everything; then every token is on its own.  Every block makes both sums by itself, 1024 requests at
-// a time, and writes an equal share of the tokens' slots; the token on the first place of a new page writes the table's entry.
-constexpr int SLOT_THREADS = 1024, SLOT_WARPS = SLOT_THREADS / 32;
+// pages) therefore say everything; then every token is on its own.  Every block makes both sums by itself, as many requests at
+// a time as it has threads, and writes an equal share of the tokens' slots; the token on the first place of a new page writes the table's entry.
+// Latency bounds it: a step of 64 requests 2.6 us (2.0 is an empty launch), prompts of 1.2 million tokens 9.1 (10 MB).
 
 struct Request {
     int old_tokens, new_tokens;
@@ -31,6 +31,7 @@ __device__ __forceinline__ Request request_of(const BlkPagedSlotsParams& p, int 
 }
 
 // Sums of the block's (tokens, pages) up to and without this thread's; *all: of the whole block.  Ends behind a barrier.
+template <int THREADS>
 __device__ __forceinline__ longlong2 block_before(longlong2 mine, longlong2* all, longlong2* sums) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     longlong2 s = mine;
@@ -45,7 +46,7 @@ __device__ __forceinline__ longlong2 block_before(longlong2 mine, longlong2* all
     if (lane == 31) sums[warp] = s;
     __syncthreads();
     if (warp == 0) {
-        longlong2 t = sums[lane];
+        longlong2 t = lane < THREADS / 32 ? sums[lane] : make_longlong2(0, 0);
 #pragma unroll
         for (int x = 1; x < 32; x *= 2) {
             const long long a = __shfl_up_sync(0xffffffffu, t.x, x), b = __shfl_up_sync(0xffffffffu, t.y, x);
@@ -54,10 +55,10 @@ __device__ __forceinline__ longlong2 block_before(longlong2 mine, longlong2* all
                 t.y += b;
             }
         }
-        sums[lane] = t;
+        if (lane < THREADS / 32) sums[lane] = t;
     }
     __syncthreads();
-    *all = sums[SLOT_WARPS - 1];
+    *all = sums[THREADS / 32 - 1];
     if (warp) {
         s.x += sums[warp - 1].x;
         s.y += sums[warp - 1].y;
@@ -68,7 +69,9 @@ __device__ __forceinline__ longlong2 block_before(longlong2 mine, longlong2* all
 }
 __device__ __forceinline__ int saturated(long long x) { return (int)min(x, (long long)INT_MAX); }
 
+template <int SLOT_THREADS>
 __global__ void __launch_bounds__(SLOT_THREADS) blk_paged_slots_kernel(const BlkPagedSlotsParams p) {
+    constexpr int SLOT_WARPS = SLOT_THREADS / 32;
     __shared__ longlong2 sums[SLOT_WARPS];
     __shared__ long long s_start[SLOT_THREADS + 1], s_page[SLOT_THREADS];
     __shared__ int s_old[SLOT_THREADS];
@@ -76,13 +79,13 @@ __global__ void __launch_bounds__(SLOT_THREADS) blk_paged_slots_kernel(const Blk
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     blk_grid_wait();
     const int taken = max(p.taken[0], 0);
-    long long tokens = 0, pages = taken;  // of the requests before this thousand
+    long long tokens = 0, pages = taken;  // of the requests before these
     for (int base = 0; base < p.requests; base += SLOT_THREADS) {
         const int r = base + tid, here = min(SLOT_THREADS, p.requests - base);
         Request q{0, 0, 0, 0};
         if (r < p.requests) q = request_of(p, r);
         longlong2 all;
-        const longlong2 before = block_before(make_longlong2(q.new_tokens, q.pages), &all, sums);
+        const longlong2 before = block_before<SLOT_THREADS>(make_longlong2(q.new_tokens, q.pages), &all, sums);
         s_start[tid] = before.x;
         s_page[tid] = pages + before.y;
         s_old[tid] = q.old_tokens;
@@ -132,17 +135,18 @@ __global__ void __launch_bounds__(SLOT_THREADS) blk_paged_slots_kernel(const Blk
 }
 
 // What a call of many blocks leaves for the end when the lengths it reads are to be advanced in place.
-__global__ void __launch_bounds__(SLOT_THREADS) blk_paged_advance_kernel(const BlkPagedSlotsParams p) {
-    __shared__ longlong2 sums[SLOT_WARPS];
+constexpr int MANY = 1024, SOME = 256;  // threads of a block
+__global__ void __launch_bounds__(MANY) blk_paged_advance_kernel(const BlkPagedSlotsParams p) {
+    __shared__ longlong2 sums[MANY / 32];
     blk_grid_wait();
     long long pages = 0;
-    for (int r = threadIdx.x; r < p.requests; r += SLOT_THREADS) {
+    for (int r = threadIdx.x; r < p.requests; r += MANY) {
         const Request q = request_of(p, r);
         pages += q.pages;
         p.lengths_out[r] = q.old_tokens + q.new_tokens;
     }
     longlong2 all;
-    block_before(make_longlong2(0, pages), &all, sums);
+    block_before<MANY>(make_longlong2(0, pages), &all, sums);
     if (threadIdx.x == 0) p.taken_out[0] = saturated(max(p.taken[0], 0) + all.y);
 }
 
@@ -192,9 +196,12 @@ __global__ void __launch_bounds__(APPEND_THREADS) blk_paged_append_kernel(const 
 
 }  // namespace
 
-// One block does it all for a step's few tokens: no other block's sums to repeat, and a call in place needs no second launch.
+// One block does it all for a step's few tokens: no other block's sums to repeat, and a call in place needs no second launch.  It is a small one for
+// requests and tokens of a step: 64 requests of a token each 2.6 us, by 1024 threads 3.5; 600 requests, which the small one would take in
+// three turns, 1.2 million tokens by blocks of 1024 threads 9.1, of 256 15.0.
 cudaError_t blk_launch_paged_slots(const BlkPagedSlotsParams& p_in, int sms, cudaStream_t st) {
     BlkPagedSlotsParams p = p_in;
+    if (p.requests <= SOME && p.tokens <= 4 * SOME) return blk_launch(true, blk_paged_slots_kernel<SOME>, dim3(1), dim3(SOME), (size_t)0, st, p);
     const bool in_place = p.lengths_out == p.lengths || p.taken_out == p.taken;
     const int64_t share = 8192;  // tokens that a block of its own is worth
     const int64_t want = (p.tokens + share - 1) / share;
@@ -203,9 +210,9 @@ cudaError_t blk_launch_paged_slots(const BlkPagedSlotsParams& p_in, int sms, cud
         p.lengths_out = nullptr;
         p.taken_out = nullptr;
     }
-    cudaError_t e = blk_launch(true, blk_paged_slots_kernel, dim3(blocks), dim3(SLOT_THREADS), (size_t)0, st, p);
+    cudaError_t e = blk_launch(true, blk_paged_slots_kernel<MANY>, dim3(blocks), dim3(MANY), (size_t)0, st, p);
     if (e != cudaSuccess || blocks == 1 || !in_place) return e;
-    return blk_launch(true, blk_paged_advance_kernel, dim3(1), dim3(SLOT_THREADS), (size_t)0, st, p_in);
+    return blk_launch(true, blk_paged_advance_kernel, dim3(1), dim3(MANY), (size_t)0, st, p_in);
 }
 
 cudaError_t blk_launch_paged_append(const BlkPagedAppendParams& p, cudaStream_t st) {

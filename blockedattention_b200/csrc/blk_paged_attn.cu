@@ -41,9 +41,9 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 __device__ __forceinline__ bool part_counts(float l, float top) { return l != 0.f && !(l == INFINITY && top > -INFINITY); }
 __device__ __forceinline__ float part_weight(float m, float top, float c) { return m == -INFINITY ? 1.f : blk_exp2((m - top) * c); }
 
-// Place of a column of row q among eight rows of DP floats: rows two apart lie eight banks apart, as a warp's accumulators are spread.
+// Place of a column of row q among rows of DP floats: rows two apart lie eight banks apart, as a warp's accumulators are spread.
 template <int DP>
-__device__ __forceinline__ int merge_at(int q, int col) { return q * DP + (col ^ ((q >> 1) << 3)); }
+__device__ __forceinline__ int merge_at(int q, int col) { return q * DP + (col ^ ((q >> 1 & 3) << 3)); }
 
 // ---- the arithmetic of one warp, 16-bit types ---------------------------------------------------------
 // Scores and values on the tensor cores with the tokens as the wide side: S^T = K Q^T is (16 tokens x 8 query rows), O^T = V^T P^T is
@@ -230,29 +230,34 @@ struct Math16 {
 };
 
 // ---- the same in 32 bits -------------------------------------------------------------------------------
-// A lane holds four columns (eight at 256) of q, of every token's key and value and of the result, two operations to an instruction; below 128
-// columns half a warp does, and the warp takes two tokens at once.  A token's eight scores (a sum over the lanes each) are
-// added by halves, so that 32 sums of four tokens cost 31 exchanges and end up one in each lane, where the softmax goes on.
+// A lane holds four columns (eight at 256) of q, of every token's key and value and of the result, two operations to an instruction; up to 64
+// columns half a warp does, and the warp takes two tokens at once.  A score is a sum over the lanes: R rows of several tokens are
+// added together, by halves, so that as many sums as there are lanes cost one exchange each and end up one in each lane, where the softmax
+// goes on.
 struct BlkFloatTag {};
-template <int DP_, int TW_, int STAGES_, int CTAS_, int PASS_>
+template <int DP_, int R_, int TW_, int STAGES_, int CTAS_, int PASS_>
 struct Math32 {
     typedef BlkFloatTag Tag;
-    static constexpr int DP = DP_, GU = 8, E = 4, TW = TW_, STAGES = STAGES_, CTAS = CTAS_, PASS = PASS_;
-    static constexpr int LANES = DP == 64 ? 16 : 32, C = DP / 4 / LANES, PAR = 32 / LANES, BATCHES = TW / 4;  // lanes of a token, its vectors in a lane, tokens at once
-    static constexpr int EXTRA = WARPS * TW * 8 * 4;  // every warp's weights
-    float2 q[8][C][2], o[8][C][2];
+    static constexpr int DP = DP_, R = R_, GU = R, E = 4, TW = TW_, STAGES = STAGES_, CTAS = CTAS_, PASS = PASS_ < R ? PASS_ : R;
+    static constexpr int LANES = DP == 64 ? 16 : 32, C = DP / 4 / LANES, PAR = 32 / LANES;  // lanes of a token, its vectors in a lane, tokens at once
+    static constexpr int TURNS = TW / PAR < LANES / R ? TW / PAR : LANES / R, BATCHES = TW / PAR / TURNS;  // tokens in turn that are added together
+    static constexpr int SUMS = R * TURNS, SAME = LANES / SUMS;                                          // sums; lanes that have the same one
+    static constexpr int EXTRA = WARPS * TW * R * 4;                                                     // every warp's weights
+    static_assert(TURNS * BATCHES * PAR == TW && SUMS * SAME == LANES, "powers of two");
+    float2 q[R][C][2], o[R][C][2];
     float m, l;  // of this lane's row
     bool seen;
     int d;
 
-    static __device__ __forceinline__ int row_of(int lane) { return PAR == 2 ? lane >> 1 & 7 : lane >> 2; }
-    static __device__ __forceinline__ int token_of(int lane) { return PAR == 2 ? (lane & 1) * 2 + (lane >> 4) : lane & 3; }
+    static __device__ __forceinline__ int row_of(int lane) { return lane % LANES / SAME % R; }
+    static __device__ __forceinline__ int token_of(int lane) { return lane % LANES / SAME / R * PAR + lane / LANES; }  // in a batch
     static __device__ __forceinline__ int col_of(int c, int lane) { return (c * LANES + lane % LANES) * 4; }
+    static constexpr bool of_token(int x) { return x >= SAME * R; }  // lanes that differ in bit x have other tokens of the same row
 
     __device__ __forceinline__ void fetch(const BlkPagedAttnParams& p, const char* at, int rows, int lane) {
         d = p.d;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -263,7 +268,7 @@ struct Math32 {
     }
     __device__ __forceinline__ void begin(uint32_t) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int c = 0; c < C; ++c) o[i][c][0] = o[i][c][1] = make_float2(0.f, 0.f);
         m = -INFINITY;
@@ -279,29 +284,36 @@ struct Math32 {
                      : "r"(s + x / 8 * (TW * 128) + t * 128 + (((x & 7) ^ (t & 7)) << 4)));
         return v;
     }
-    // a[0 .. 2N) of this lane and of the one that differs in bit x: the sums of the half that the bit chooses
-    template <int N>
-    static __device__ __forceinline__ void halve(const float* a, float* b, int x, int lane) {
-        const bool high = lane & x;
+    // a[0 .. N) of LANES lanes, added: sum lane / SAME in every lane
+    template <int N, int X>
+    static __device__ __forceinline__ float added(const float* a, int lane) {
+        if constexpr (N > 1) {
+            float b[N / 2];
+            const bool high = lane & X;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float keep = high ? a[i + N] : a[i], give = high ? a[i] : a[i + N];
-            b[i] = keep + __shfl_xor_sync(0xffffffffu, give, x);
+            for (int i = 0; i < N / 2; ++i) {
+                const float keep = high ? a[i + N / 2] : a[i], give = high ? a[i] : a[i + N / 2];
+                b[i] = keep + __shfl_xor_sync(0xffffffffu, give, X);
+            }
+            return added<N / 2, X / 2>(b, lane);
+        } else {
+            float s = a[0];
+#pragma unroll
+            for (int x = X; x >= 1; x /= 2) s += __shfl_xor_sync(0xffffffffu, s, x);
+            return s;
         }
     }
 
     __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, uint32_t mask, float sign, float scale, uint32_t sx, int lane) {
-        constexpr int TOP = PAR == 2 ? 8 : 16;
         seen = true;
         const int row = row_of(lane), tok = token_of(lane);
         float s[BATCHES];
 #pragma unroll
         for (int b = 0; b < BATCHES; ++b) {
-            float r[4 / PAR];
+            float a[SUMS];
 #pragma unroll
-            for (int j = 0; j < 4 / PAR; ++j) {
-                const int t = 4 * b + (PAR == 2 ? 2 * j + (lane >> 4) : j);
-                float a[8], h4[4], h2[2];
+            for (int u = 0; u < TURNS; ++u) {
+                const int t = (b * TURNS + u) * PAR + lane / LANES;
                 float4 k[C];
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
@@ -309,51 +321,43 @@ struct Math32 {
                     if (col_of(c, lane) >= d) k[c] = make_float4(0.f, 0.f, 0.f, 0.f);  // (no copy has written there)
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < R; ++i) {
                     float2 x = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
                         x = blk_fma2(make_float2(k[c].x, k[c].y), q[i][c][0], x);
                         x = blk_fma2(make_float2(k[c].z, k[c].w), q[i][c][1], x);
                     }
-                    a[i] = x.x + x.y;
+                    a[u * R + i] = x.x + x.y;
                 }
-                halve<4>(a, h4, TOP, lane);
-                halve<2>(h4, h2, TOP / 2, lane);
-                halve<1>(h2, r + j, TOP / 4, lane);
             }
-            if (PAR == 1) {
-                float h[2];
-                halve<2>(r, h, 2, lane);
-                halve<1>(h, s + b, 1, lane);
-            } else {
-                halve<1>(r, s + b, 1, lane);
-            }
-            s[b] *= sign;
+            s[b] = added<SUMS, LANES / 2>(a, lane) * sign;
         }
         float top = -INFINITY;
 #pragma unroll
         for (int b = 0; b < BATCHES; ++b)
-            if (mask >> (4 * b + tok) & 1) top = fmaxf(top, s[b]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, PAR == 2 ? 16 : 2));
+            if (mask >> (b * TURNS * PAR + tok) & 1) top = fmaxf(top, s[b]);
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2)
+            if (of_token(x)) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
         top = fmaxf(top, m);
         const float ref = top == -INFINITY ? 0.f : top, alpha = blk_exp2((m - ref) * scale);
         const bool grew = __any_sync(0xffffffffu, top > m);
         m = top;
-        const uint32_t sp = sx + (threadIdx.x / 32) * (TW * 8 * 4);
+        const uint32_t sp = sx + (threadIdx.x / 32) * (TW * R * 4);
         if (grew) l *= alpha;
         __syncwarp();  // (the weights of the tile before are read)
 #pragma unroll
         for (int b = 0; b < BATCHES; ++b) {
-            const float w = mask >> (4 * b + tok) & 1 ? blk_exp2((s[b] - ref) * scale) : 0.f;
+            const int t = b * TURNS * PAR + tok;
+            const float w = mask >> t & 1 ? blk_exp2((s[b] - ref) * scale) : 0.f;
             l += w;
-            blk_sts_f32(sp + ((4 * b + tok) * 8 + row) * 4, w);
+            blk_sts_f32(sp + (t * R + row) * 4, w);
         }
         if (grew) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = __shfl_sync(0xffffffffu, alpha, i * (PAR == 2 ? 2 : 4));
+            for (int i = 0; i < R; ++i) {
+                const float x = __shfl_sync(0xffffffffu, alpha, i * SAME);
 #pragma unroll
                 for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -363,18 +367,16 @@ struct Math32 {
         __syncwarp();
 #pragma unroll 4
         for (int u = 0; u < TW / PAR; ++u) {
-            const int t = PAR == 2 ? 2 * u + (lane >> 4) : u;
-            float w[8];
+            const int t = u * PAR + lane / LANES;
+            float w[R];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n"
-                             : "=f"(w[4 * i]), "=f"(w[4 * i + 1]), "=f"(w[4 * i + 2]), "=f"(w[4 * i + 3])
-                             : "r"(sp + t * 32 + i * 16));
+            for (int i = 0; i < R / 2; ++i)
+                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];\n" : "=f"(w[2 * i]), "=f"(w[2 * i + 1]) : "r"(sp + (t * R + 2 * i) * 4));
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const float4 v = vec(sV, t, c, lane);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < R; ++i) {
                     o[i][c][0] = blk_fma2(make_float2(w[i], w[i]), make_float2(v.x, v.y), o[i][c][0]);
                     o[i][c][1] = blk_fma2(make_float2(w[i], w[i]), make_float2(v.z, v.w), o[i][c][1]);
                 }
@@ -384,8 +386,9 @@ struct Math32 {
 
     __device__ __forceinline__ void stats(float* sm, float* sl, int lane) {
         float t = l;
-        t += __shfl_xor_sync(0xffffffffu, t, 1);
-        t += __shfl_xor_sync(0xffffffffu, t, PAR == 2 ? 16 : 2);
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2)
+            if (of_token(x)) t += __shfl_xor_sync(0xffffffffu, t, x);
         if (token_of(lane) == 0) {
             sm[row_of(lane)] = m;
             sl[row_of(lane)] = seen && t == 0.f ? INFINITY : t;
@@ -393,7 +396,7 @@ struct Math32 {
     }
     __device__ __forceinline__ void put(int n, float* dst, int rows, int lane) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < R; ++i)
             if (i / PASS == n && i < rows) {
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
@@ -491,15 +494,17 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     }
     blk_grid_wait();
 
-    // The lengths, added up: a run of requests for every thread.  A range is cut by cost: to change heads costs three quarters of a tile.  Tile t of
-    // a head begins at cost 0 for t = 0, else HEAD + TIME t, and belongs to the block whose range this lies in.  With less than
-    // a head of one tile for every block tiles alone count, so that none is empty.
+    // The lengths, added up: a run of requests for every thread, by each half of the block for itself.  A block's range is cut by cost: to change
+    // heads costs three quarters of a tile.  Tile t of a head begins at cost 0 for t = 0, else HEAD + TIME t, and belongs to the block whose range
+    // this lies in.  With less than a head of one tile for every block tiles alone count, so that none is empty.
     Walk cw{};
-    int64_t all, blocks, first;  // cost of everything; blocks that have a part of it; this one's first tile
+    int64_t each, over, blocks, first;  // range c: from cost c each + min(c, over) on; blocks that have one; this one's first tile
     int64_t count;
     int TIME = 4, HEAD = 3;
     {
-        const int per = (p.requests + THREADS - 1) / THREADS, r0 = min(tid * per, p.requests), r1 = min(r0 + per, p.requests);
+        constexpr int HALF = THREADS / 2, HW = WARPS / 2;
+        const int e = tid / HALF, ht = tid % HALF;  // the half finds the beginning (0) or the end (1) of the range
+        const int per = (p.requests + HALF - 1) / HALF, r0 = min(ht * per, p.requests), r1 = min(r0 + per, p.requests);
         int64_t mine = 0;
         for (int r = r0; r < r1; ++r) mine += tiles_of<TILE>(held(p, r));
         int64_t before = mine;
@@ -512,28 +517,29 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         __syncthreads();
         int64_t tiles = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) before += sched[w];
-            tiles += sched[w];
+        for (int w = 0; w < HW; ++w) {
+            const int64_t y = sched[w];
+            if (w < warp % HW) before += y;
+            tiles += y;
         }
         before -= mine;
         blocks = gridDim.x;
-        if (p.units * (TIME * tiles + HEAD * (int64_t)p.requests) < blocks * (TIME + HEAD)) {
+        int64_t all = p.units * (TIME * tiles + HEAD * (int64_t)p.requests);  // the cost of everything
+        if (all < blocks * (TIME + HEAD)) {
             TIME = 1;
             HEAD = 0;
-            blocks = min(blocks, p.units * tiles);
+            all = p.units * tiles;
+            blocks = min(blocks, all);
         }
         if (blockIdx.x >= blocks) {
             if (tid == 0) p.parts[blockIdx.x] = make_int4(0, 0, 0, 0);
             return;
         }
-        all = p.units * (TIME * tiles + HEAD * (int64_t)p.requests);
-        // the two ends of the range, by the thread that has the request which each lies in
+        each = quotient(all, blocks);
+        over = all - each * blocks;
+        const int64_t x = (blockIdx.x + e) * each + min((int64_t)blockIdx.x + e, over);
         const int64_t lo_cost = p.units * (TIME * before + HEAD * (int64_t)r0), hi_cost = lo_cost + p.units * (TIME * mine + HEAD * (int64_t)(r1 - r0));
-#pragma unroll 1
-        for (int e = 0; e < 2; ++e) {
-            const int64_t x = quotient((blockIdx.x + e) * all, blocks);
-            if (x < lo_cost || x >= hi_cost) continue;
+        if (x >= lo_cost && x < hi_cost) {
             int64_t at = lo_cost, tile = before;
             int r = r0, len, n;
             for (;; ++r) {
@@ -544,20 +550,19 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
                 at = end;
                 tile += n;
             }
-            const int64_t span = (int64_t)TIME * n + HEAD, unit = quotient(x - at, span);
-            const int y = (int)(x - at - unit * span), t = y == 0 ? 0 : max(1, (y - HEAD + TIME - 1) / TIME);  // t = n: the next head's first
-            sched[8 + 4 * e] = p.units * tile + unit * n + t;
-            if (e == 0) {
-                sched[9] = r;
-                sched[10] = len;
-                sched[11] = unit;
-                sched[13] = t;
-            }
+            const int64_t span = (int64_t)TIME * n + HEAD, unit = p.units == 1 ? 0 : quotient(x - at, span);
+            const int y = (int)(x - at - unit * span);
+            const int t = y == 0 ? 0 : TIME == 1 ? y : max(1, (y - HEAD + TIME - 1) / 4);  // t = n: the next head's first
+            sched[8 + 8 * e] = p.units * tile + unit * n + t;
+            sched[9 + 8 * e] = r;
+            sched[10 + 8 * e] = len;
+            sched[11 + 8 * e] = unit;
+            sched[12 + 8 * e] = t;
         }
-        if (tid == 0 && blockIdx.x + 1 == blocks) sched[12] = p.units * tiles;
+        if (tid == 0 && blockIdx.x + 1 == blocks) sched[16] = p.units * tiles;
         __syncthreads();
         first = sched[8];
-        count = sched[12] - first;
+        count = sched[16] - first;
         cw.r = (int)sched[9];
         if (cw.r + 1 < p.requests) cw.ahead = p.lengths[cw.r + 1];
         cw.len = (int)sched[10];
@@ -565,7 +570,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         const int unit = (int)sched[11];
         cw.kv = p.q_units == 1 ? unit : unit / p.q_units;
         cw.part = unit - cw.kv * p.q_units;
-        cw.t = (int)sched[13];
+        cw.t = (int)sched[12];
         if (cw.t == cw.n) {
             cw.t -= 1;
             step<TILE>(cw, p);
@@ -576,6 +581,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     auto q_at = [&](const Walk& w) { return p.q + w.r * p.q_row_stride + (int64_t)(w.kv * p.group + w.part * p.rows_unit) * p.q_head_stride; };
     auto rows_at = [&](const Walk& w) { return min(p.rows_unit, p.group - w.part * p.rows_unit); };
     math.fetch(p, q_at(cw), rows_at(cw), lane);
+
     // Copies.  Where pages are whole numbers of a warp's tokens (one_page), these lie side by side on one page; else a lane looks up the page of one
     // of them.  That is done two tiles before the rows are asked for; eight lanes take 128 bytes of a row.
     Walk pw = cw;
@@ -743,7 +749,8 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
             if (begins && !ends) {  // the head goes on in the blocks up to the one that has its last tile
                 const int64_t tile = first + i - now.t, head = (int64_t)now.r * p.units + now.kv * p.q_units + now.part;  // its first tile; heads before it
                 const int64_t last = TIME * (tile + now.n - 1) + HEAD * (head + 1);  // (of two tiles or more)
-                part = make_int4((int)quotient((last + 1) * blocks - 1, all) - (int)blockIdx.x + 1, now.r, now.kv, now.part);
+                const int64_t wide = over * (each + 1), owner = last < wide ? quotient(last, each + 1) : over + quotient(last - wide, each);
+                part = make_int4((int)owner - (int)blockIdx.x + 1, now.r, now.kv, now.part);
             }
             if (more) math.begin(extra);
         }
@@ -752,129 +759,153 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     if (tid == 0) p.parts[blockIdx.x] = part;
 }
 
-// Joins the parts of the heads that were cut.  Every block finds these heads for itself, then takes rows of them in turn: a part for
-// every warp, its statistics and values asked for together, then the warps' results as parts again.
-constexpr int JOIN_WARPS = 8, MAX_BLOCKS = 1024;
-template <typename Tag, int DP>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const BlkPagedAttnParams p, int GU, int blocks, float out_scale) {
-    constexpr int V = DP % 128 == 0 ? 4 : DP % 64 == 0 ? 2 : 1, W = DP / 32 / V;  // vectors of V floats, W of them for a lane
-    __shared__ __align__(16) float values[JOIN_WARPS][DP];
-    __shared__ float tops[JOIN_WARPS], sums[JOIN_WARPS];
-    __shared__ uint32_t cut[MAX_BLOCKS / 32];
-    __shared__ int4 heads[MAX_BLOCKS];  // of those that were cut: parts, request, key head, part of its rows
-    __shared__ int begins[MAX_BLOCKS];  // the block that each begins in
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    blk_grid_wait();
-    constexpr int AT_ONCE = 2;
-    int total = 0;
-    for (int base = 0; base < blocks; base += JOIN_WARPS * 32 * AT_ONCE) {
-        int4 part[AT_ONCE];
+// Joins the parts of the heads that were cut.  Every warp looks through the blocks' notes for these heads.  Heads of few parts are rows for
+// warps, the others for blocks: a part for every warp, then the warps' results as parts again.  A part's statistics and values are asked
+// for together.
+constexpr int JOIN_WARPS = 8, MAX_BLOCKS = 512, FEW = 8;
+template <int DP>
+struct Joined {
+    static constexpr int W = (DP / 4 + 31) / 32;  // vectors of a row in a lane
+    float top, sum;
+    float4 v[W];
+    __device__ __forceinline__ void begin() {
+        top = -INFINITY;
+        sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            const int c = base + j * (JOIN_WARPS * 32) + tid;
-            part[j] = c < blocks ? p.parts[c] : make_int4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            const uint32_t word = __ballot_sync(0xffffffffu, part[j].x != 0);
-            if (lane == 0) cut[j * JOIN_WARPS + warp] = word;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            int rank = total;
-            for (int w = 0; w < j * JOIN_WARPS + warp; ++w) rank += __popc(cut[w]);
-            rank += __popc(cut[j * JOIN_WARPS + warp] & ((1u << lane) - 1));
-            if (part[j].x) {
-                heads[rank] = part[j];
-                begins[rank] = base + j * (JOIN_WARPS * 32) + tid;
-            }
-        }
-        for (int w = 0; w < AT_ONCE * JOIN_WARPS; ++w) total += __popc(cut[w]);
-        __syncthreads();
+        for (int w = 0; w < W; ++w) v[w] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const int64_t size = GU * DP + 2 * GU;
-    for (int item = blockIdx.x; item < total * p.rows_unit; item += gridDim.x) {
-        const int which = item / p.rows_unit, row = item - which * p.rows_unit;
-        const int4 head = heads[which];
-        const int rows = min(p.rows_unit, p.group - head.w * p.rows_unit);
-        if (row >= rows) continue;
-        const float* const base = p.work + 2 * (int64_t)begins[which] * size;  // part i > 0 is the first of block c + i
-        float top = -INFINITY, sum = 0.f, acc[W][V];
+    // parts first, first + step, ... N of them at the most
+    template <int N, typename A>
+    __device__ __forceinline__ void add(const BlkPagedAttnParams& p, A at, int GU, int row, int first, int step, int end, int lane) {
+        float m[N], l[N];
+        float4 y[N][W];
 #pragma unroll
-        for (int j = 0; j < W; ++j)
+        for (int j = 0; j < N; ++j) {
+            m[j] = -INFINITY;
+            l[j] = 0.f;
+            if (first + j * step >= end) continue;
+            const float* a = at(first + j * step);
+            m[j] = a[GU * DP + row];
+            l[j] = a[GU * DP + GU + row];
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[j][e] = 0.f;
-        auto add = [&](float m, float l, const float (&y)[W][V]) {
-            const float up = fmaxf(top, m);
-            if (!part_counts(l, up)) return;  // (the same for the whole warp)
-            const bool before = part_counts(sum, up);
-            const float old = part_weight(top, up, p.c), w = part_weight(m, up, p.c);
-            sum = before ? fmaf(sum, old, w * l) : w * l;
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-#pragma unroll
-                for (int e = 0; e < V; ++e) acc[j][e] = before ? fmaf(acc[j][e], old, w * y[j][e]) : w * y[j][e];
-            top = up;
-        };
-        constexpr int N = 4;
-        for (int i = warp; i < head.x; i += JOIN_WARPS * N) {
-            float m[N], l[N], y[N][W][V];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int k = i + j * JOIN_WARPS;
-                const float* at = base + (2 * (int64_t)k + (k == 0)) * size;
-                m[j] = -INFINITY;
-                l[j] = 0.f;
-                if (k >= head.x) continue;
-                m[j] = at[GU * DP + row];
-                l[j] = at[GU * DP + GU + row];
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const int col = (w * 32 + lane) * V;
-                    const float* from = at + row * DP + col;
-                    if (V == 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(from);
-                        y[j][w][0] = x.x, y[j][w][1 % V] = x.y, y[j][w][2 % V] = x.z, y[j][w][3 % V] = x.w;
-                    } else if (V == 2) {
-                        const float2 x = *reinterpret_cast<const float2*>(from);
-                        y[j][w][0] = x.x, y[j][w][1 % V] = x.y;
-                    } else {
-                        y[j][w][0] = *from;
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) add(m[j], l[j], y[j]);
+            for (int w = 0; w < W; ++w)
+                if ((w * 32 + lane) * 4 < p.d) y[j][w] = *reinterpret_cast<const float4*>(a + row * DP + (w * 32 + lane) * 4);
         }
+        float up = top;
+#pragma unroll
+        for (int j = 0; j < N; ++j) up = fmaxf(up, m[j]);
+        const bool before = part_counts(sum, up);
+        const float old = part_weight(top, up, p.c);
+        sum = before ? sum * old : 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[w] = before ? make_float4(v[w].x * old, v[w].y * old, v[w].z * old, v[w].w * old) : make_float4(0.f, 0.f, 0.f, 0.f);
+        top = up;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (!part_counts(l[j], up)) continue;  // (the same for the whole warp)
+            const float f = part_weight(m[j], up, p.c);
+            sum = fmaf(f, l[j], sum);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                v[w].x = fmaf(f, y[j][w].x, v[w].x);
+                v[w].y = fmaf(f, y[j][w].y, v[w].y);
+                v[w].z = fmaf(f, y[j][w].z, v[w].z);
+                v[w].w = fmaf(f, y[j][w].w, v[w].w);
+            }
+        }
+    }
+    template <typename Tag>
+    __device__ __forceinline__ void write(const BlkPagedAttnParams& p, int64_t head, float out_scale, int lane) const {
 #pragma unroll
         for (int w = 0; w < W; ++w)
+            if ((w * 32 + lane) * 4 < p.d) Out<Tag>::put4(p.out, head * p.d + (w * 32 + lane) * 4, divided(v[w], sum, out_scale));
+        if (p.lse && lane == 0) p.lse[head] = row_log(top, sum, p.scale);
+    }
+};
+
+template <typename Tag, int DP>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const BlkPagedAttnParams p, int GU, int blocks, float out_scale) {
+    constexpr int W = Joined<DP>::W;
+    __shared__ __align__(16) float values[JOIN_WARPS][W * 128];
+    __shared__ float stats[JOIN_WARPS][2];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    blk_grid_wait();
+    uint32_t few[MAX_BLOCKS / 32], many[MAX_BLOCKS / 32];  // blocks that a cut head of few, of many parts begins in
+    int num_few = 0, num_many = 0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) values[warp][(w * 32 + lane) * V + e] = acc[w][e];
+    for (int k = 0; k < MAX_BLOCKS / 32; ++k) few[k] = k * 32 + lane < blocks ? (uint32_t)p.parts[k * 32 + lane].x : 0u;
+#pragma unroll
+    for (int k = 0; k < MAX_BLOCKS / 32; ++k) {
+        const uint32_t n = few[k];
+        few[k] = __ballot_sync(0xffffffffu, n > 0 && n <= FEW);
+        many[k] = __ballot_sync(0xffffffffu, n > FEW);
+        num_few += __popc(few[k]);
+        num_many += __popc(many[k]);
+    }
+    // block number `left` of a set (the same for the whole warp)
+    auto find = [&](const uint32_t (&set)[MAX_BLOCKS / 32], int left) {
+        uint32_t word = 0;
+        int base = 0, rank = -1;
+#pragma unroll
+        for (int k = 0; k < MAX_BLOCKS / 32; ++k) {
+            const int n = __popc(set[k]);
+            if (left >= 0 && left < n) {
+                word = set[k];
+                base = k * 32;
+                rank = left;
+            }
+            left -= n;
+        }
+        const bool here = (word >> lane & 1) && __popc(word & ((1u << lane) - 1)) == rank;
+        return base + __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    };
+    const int64_t size = GU * (DP + 2);
+    Joined<DP> sum;
+    for (int item = blockIdx.x + warp * gridDim.x; item < num_few * p.rows_unit; item += gridDim.x * JOIN_WARPS) {
+        const int which = item / p.rows_unit, row = item - which * p.rows_unit, c = find(few, which);
+        const int4 head = p.parts[c];  // parts, request, key head, part of its rows
+        if (row >= min(p.rows_unit, p.group - head.w * p.rows_unit)) continue;
+        sum.begin();
+        sum.template add<FEW>(p, [&](int i) { return p.work + (2 * (int64_t)(c + i) + (i == 0)) * size; }, GU, row, 0, 1, head.x, lane);
+        sum.template write<Tag>(p, (int64_t)head.y * p.heads + head.z * p.group + head.w * p.rows_unit + row, out_scale, lane);
+    }
+    for (int item = blockIdx.x; item < num_many * p.rows_unit; item += gridDim.x) {
+        const int which = item / p.rows_unit, row = item - which * p.rows_unit, c = find(many, which);
+        const int4 head = p.parts[c];
+        if (row >= min(p.rows_unit, p.group - head.w * p.rows_unit)) continue;
+        auto at = [&](int i) { return p.work + (2 * (int64_t)(c + i) + (i == 0)) * size; };
+        constexpr int N = 4;
+        sum.begin();
+        for (int i = warp; i < head.x; i += JOIN_WARPS * N) sum.template add<N>(p, at, GU, row, i, JOIN_WARPS, head.x, lane);
+#pragma unroll
+        for (int w = 0; w < W; ++w) *reinterpret_cast<float4*>(&values[warp][(w * 32 + lane) * 4]) = sum.v[w];
         if (lane == 0) {
-            tops[warp] = top;
-            sums[warp] = sum;
+            stats[warp][0] = sum.top;
+            stats[warp][1] = sum.sum;
         }
         __syncthreads();
-        if (tid * 4 < p.d) {
-            float t = -INFINITY, l = 0.f;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (warp == 0) {
+            float top = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < JOIN_WARPS; ++w) t = fmaxf(t, tops[w]);
+            for (int k = 0; k < JOIN_WARPS; ++k) top = fmaxf(top, stats[k][0]);
+            sum.begin();
 #pragma unroll
-            for (int w = 0; w < JOIN_WARPS; ++w)
-                if (part_counts(sums[w], t)) {
-                    const float f = part_weight(tops[w], t, p.c);
-                    const float4 y = *reinterpret_cast<const float4*>(&values[w][tid * 4]);
-                    l = fmaf(f, sums[w], l);
-                    v.x = fmaf(f, y.x, v.x);
-                    v.y = fmaf(f, y.y, v.y);
-                    v.z = fmaf(f, y.z, v.z);
-                    v.w = fmaf(f, y.w, v.w);
+            for (int k = 0; k < JOIN_WARPS; ++k) {
+                if (!part_counts(stats[k][1], top)) continue;
+                const float f = part_weight(stats[k][0], top, p.c);
+                l = fmaf(f, stats[k][1], l);
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float4 y = *reinterpret_cast<const float4*>(&values[k][(w * 32 + lane) * 4]);
+                    sum.v[w].x = fmaf(f, y.x, sum.v[w].x);
+                    sum.v[w].y = fmaf(f, y.y, sum.v[w].y);
+                    sum.v[w].z = fmaf(f, y.z, sum.v[w].z);
+                    sum.v[w].w = fmaf(f, y.w, sum.v[w].w);
                 }
-            const int64_t at = (int64_t)head.y * p.heads + head.z * p.group + head.w * p.rows_unit + row;
-            Out<Tag>::put4(p.out, at * p.d + tid * 4, divided(v, l, out_scale));
-            if (p.lse && tid == 0) p.lse[at] = row_log(t, l, p.scale);
+            }
+            sum.top = top;
+            sum.sum = l;
+            sum.template write<Tag>(p, (int64_t)head.y * p.heads + head.z * p.group + head.w * p.rows_unit + row, out_scale, lane);
         }
         __syncthreads();
     }
@@ -882,40 +913,46 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const B
 
 // The kernels: padded head dimension, query rows of a unit in eights, stages, blocks on an SM, rows put together at a time.
 template <typename Tag> struct Kernels16 {
-    typedef Math16<Tag, 64, 1, 4, 3, 8> D64N1;
-    typedef Math16<Tag, 64, 2, 4, 3, 8> D64N2;
-    typedef Math16<Tag, 64, 3, 4, 2, 8> D64N3;
-    typedef Math16<Tag, 64, 4, 4, 2, 8> D64N4;
-    typedef Math16<Tag, 96, 1, 3, 2, 8> D96N1;
-    typedef Math16<Tag, 96, 2, 3, 2, 8> D96N2;
-    typedef Math16<Tag, 128, 1, 3, 2, 8> D128N1;
+    typedef Math16<Tag, 64, 1, 3, 3, 8> D64N1;
+    typedef Math16<Tag, 64, 2, 3, 3, 16> D64N2;
+    typedef Math16<Tag, 64, 3, 4, 2, 24> D64N3;
+    typedef Math16<Tag, 64, 4, 4, 2, 32> D64N4;
+    typedef Math16<Tag, 96, 1, 2, 3, 4> D96N1;
+    typedef Math16<Tag, 96, 2, 2, 2, 16> D96N2;
+    typedef Math16<Tag, 128, 1, 2, 3, 4> D128N1;
     typedef Math16<Tag, 128, 2, 3, 2, 8> D128N2;
     typedef Math16<Tag, 192, 1, 2, 2, 4> D192N1;
     typedef Math16<Tag, 256, 1, 3, 1, 4> D256N1;
 };
-typedef Math32<64, 16, 3, 2, 8> F64;
-typedef Math32<128, 8, 3, 2, 4> F128;
-typedef Math32<256, 8, 3, 1, 4> F256;
+template <int R> struct Kernels32 {
+    typedef Math32<64, R, 16, 3, 2, 8> D64;
+    typedef Math32<128, R, 8, 3, 2, 4> D128;
+    typedef Math32<256, R, 8, 3, 1, 4> D256;
+};
 
 // f(the kernel's type) for what a call needs
 template <typename M> struct Of { typedef M T; };
 template <typename F>
-auto with_kernel(int dtype, int DP, int NT, F f) {
+auto with_kernel(int dtype, int DP, int rows, F f) {
     auto half = [&](auto tag) {
         typedef Kernels16<decltype(tag)> K;
         if (DP == 64) {
-            if (NT == 1) return f(Of<typename K::D64N1>{});
-            if (NT == 2) return f(Of<typename K::D64N2>{});
-            if (NT == 3) return f(Of<typename K::D64N3>{});
+            if (rows <= 8) return f(Of<typename K::D64N1>{});
+            if (rows <= 16) return f(Of<typename K::D64N2>{});
+            if (rows <= 24) return f(Of<typename K::D64N3>{});
             return f(Of<typename K::D64N4>{});
         }
-        if (DP == 96) return NT == 1 ? f(Of<typename K::D96N1>{}) : f(Of<typename K::D96N2>{});
-        if (DP == 128) return NT == 1 ? f(Of<typename K::D128N1>{}) : f(Of<typename K::D128N2>{});
+        if (DP == 96) return rows <= 8 ? f(Of<typename K::D96N1>{}) : f(Of<typename K::D96N2>{});
+        if (DP == 128) return rows <= 8 ? f(Of<typename K::D128N1>{}) : f(Of<typename K::D128N2>{});
         return DP == 192 ? f(Of<typename K::D192N1>{}) : f(Of<typename K::D256N1>{});
+    };
+    auto full = [&](auto kernels) {
+        typedef decltype(kernels) K;
+        return DP == 64 ? f(Of<typename K::D64>{}) : DP == 128 ? f(Of<typename K::D128>{}) : f(Of<typename K::D256>{});
     };
     if (dtype == BLK_F16) return half(BlkHalfTag{});
     if (dtype == BLK_BF16) return half(BlkBf16Tag{});
-    return DP == 64 ? f(Of<F64>{}) : DP == 128 ? f(Of<F128>{}) : f(Of<F256>{});
+    return rows <= 2 ? full(Kernels32<2>{}) : rows <= 4 ? full(Kernels32<4>{}) : full(Kernels32<8>{});
 }
 
 }  // namespace
@@ -929,23 +966,22 @@ BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int
     const int most = dtype == BLK_F32 ? 8 : s.DP == 64 ? 32 : s.DP <= 128 ? 16 : 8;
     s.q_units = (group + most - 1) / most;
     s.rows_unit = (group + s.q_units - 1) / s.q_units;
-    s.NT = (s.rows_unit + 7) / 8;
     int tile = 0, ctas = 0;
-    with_kernel(dtype, s.DP, s.NT, [&](auto m) {
+    with_kernel(dtype, s.DP, s.rows_unit, [&](auto m) {
         typedef typename decltype(m)::T M;
         tile = Lay<M>::TILE;
         ctas = M::CTAS;
+        s.GU = M::GU;
     });
     const int64_t tiles = capacity > 0 ? (capacity + tile - 1) / tile : 1, room = std::min(ctas * sms, MAX_BLOCKS);
     const int64_t units = requests * kv_heads * s.q_units;
     s.blocks = (int)(units >= room || tiles >= room || units * tiles >= room ? room : units * tiles);
-    s.work_floats = (int64_t)s.blocks * 2 * (8 * s.NT) * (s.DP + 2);
+    s.work_floats = (int64_t)s.blocks * 2 * s.GU * (s.DP + 2);
     return s;
 }
 
 cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p_in, const BlkPagedShape& s, int dtype, int sms, cudaStream_t st) {
-    const int GU = 8 * s.NT;
-    return with_kernel(dtype, s.DP, s.NT, [&](auto m) {
+    return with_kernel(dtype, s.DP, s.rows_unit, [&](auto m) {
         typedef typename decltype(m)::T M;
         BlkPagedAttnParams p = p_in;
         p.one_page = p.page.d % M::TW == 0;
@@ -954,8 +990,8 @@ cudaError_t blk_launch_paged_attn(const BlkPagedAttnParams& p_in, const BlkPaged
         if (e != cudaSuccess) return e;
         e = blk_launch(true, kern, dim3((unsigned)s.blocks), dim3(THREADS), (size_t)Lay<M>::BYTES, st, p);
         if (e != cudaSuccess || s.blocks == 1) return e;
-        const int items = (s.blocks - 1) * s.rows_unit, most = 4 * sms;
+        const int items = (s.blocks - 1) * s.rows_unit, most = 2 * sms;
         return blk_launch(true, blk_paged_join_kernel<typename M::Tag, M::DP>, dim3((unsigned)(items < most ? items : most)), dim3(JOIN_WARPS * 32),
-                          (size_t)0, st, p, GU, s.blocks, M::OUT_SCALE);
+                          (size_t)0, st, p, s.GU, s.blocks, M::OUT_SCALE);
     });
 }
