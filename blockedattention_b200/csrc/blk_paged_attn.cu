@@ -830,38 +830,53 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const B
     __shared__ float stats[JOIN_WARPS][2];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     blk_grid_wait();
-    uint32_t few[MAX_BLOCKS / 32], many[MAX_BLOCKS / 32];  // blocks that a cut head of few, of many parts begins in
-    int num_few = 0, num_many = 0;
+    // the blocks that a cut head of few, of many parts begins in: 32 to a word, a word (of each kind) to a lane, and how many come before
+    constexpr int WORDS = MAX_BLOCKS / 32, EACH = WORDS / JOIN_WARPS;
+    static_assert(WORDS <= 32 && WORDS % JOIN_WARPS == 0, "a word to a lane");
+    __shared__ uint32_t words[2][WORDS];
+    {
+        int n[EACH];
 #pragma unroll
-    for (int k = 0; k < MAX_BLOCKS / 32; ++k) few[k] = k * 32 + lane < blocks ? (uint32_t)p.parts[k * 32 + lane].x : 0u;
-#pragma unroll
-    for (int k = 0; k < MAX_BLOCKS / 32; ++k) {
-        const uint32_t n = few[k];
-        few[k] = __ballot_sync(0xffffffffu, n > 0 && n <= FEW);
-        many[k] = __ballot_sync(0xffffffffu, n > FEW);
-        num_few += __popc(few[k]);
-        num_many += __popc(many[k]);
-    }
-    // block number `left` of a set (the same for the whole warp)
-    auto find = [&](const uint32_t (&set)[MAX_BLOCKS / 32], int left) {
-        uint32_t word = 0;
-        int base = 0, rank = -1;
-#pragma unroll
-        for (int k = 0; k < MAX_BLOCKS / 32; ++k) {
-            const int n = __popc(set[k]);
-            if (left >= 0 && left < n) {
-                word = set[k];
-                base = k * 32;
-                rank = left;
-            }
-            left -= n;
+        for (int k = 0; k < EACH; ++k) {
+            const int c = (warp * EACH + k) * 32 + lane;
+            n[k] = c < blocks ? p.parts[c].x : 0;
         }
-        const bool here = (word >> lane & 1) && __popc(word & ((1u << lane) - 1)) == rank;
-        return base + __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            words[0][warp * EACH + k] = __ballot_sync(0xffffffffu, n[k] > 0 && n[k] <= FEW);
+            words[1][warp * EACH + k] = __ballot_sync(0xffffffffu, n[k] > FEW);
+        }
+    }
+    __syncthreads();
+    struct Set {
+        uint32_t word;
+        int before, total;
     };
+    auto read = [&](int kind) {
+        Set s;
+        s.word = lane < WORDS ? words[kind][lane] : 0u;
+        s.before = __popc(s.word);
+#pragma unroll
+        for (int x = 1; x < WORDS; x *= 2) {
+            const int y = __shfl_up_sync(0xffffffffu, s.before, x);
+            if (lane >= x) s.before += y;
+        }
+        s.total = __shfl_sync(0xffffffffu, s.before, WORDS - 1);
+        s.before -= __popc(s.word);
+        return s;
+    };
+    // block number i of a set (the same for the whole warp)
+    auto find = [&](const Set& s, int i) {
+        const int at = __ffs(__ballot_sync(0xffffffffu, i >= s.before && i < s.before + __popc(s.word))) - 1;
+        const uint32_t word = __shfl_sync(0xffffffffu, s.word, at);
+        const int rank = i - __shfl_sync(0xffffffffu, s.before, at);
+        const bool here = (word >> lane & 1) && __popc(word & ((1u << lane) - 1)) == rank;
+        return at * 32 + __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    };
+    const Set few = read(0), many = read(1);
     const int64_t size = GU * (DP + 2);
     Joined<DP> sum;
-    for (int item = blockIdx.x + warp * gridDim.x; item < num_few * p.rows_unit; item += gridDim.x * JOIN_WARPS) {
+    for (int item = blockIdx.x + warp * gridDim.x; item < few.total * p.rows_unit; item += gridDim.x * JOIN_WARPS) {
         const int which = item / p.rows_unit, row = item - which * p.rows_unit, c = find(few, which);
         const int4 head = p.parts[c];  // parts, request, key head, part of its rows
         if (row >= min(p.rows_unit, p.group - head.w * p.rows_unit)) continue;
@@ -869,7 +884,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const B
         sum.template add<FEW>(p, [&](int i) { return p.work + (2 * (int64_t)(c + i) + (i == 0)) * size; }, GU, row, 0, 1, head.x, lane);
         sum.template write<Tag>(p, (int64_t)head.y * p.heads + head.z * p.group + head.w * p.rows_unit + row, out_scale, lane);
     }
-    for (int item = blockIdx.x; item < num_many * p.rows_unit; item += gridDim.x) {
+    for (int item = blockIdx.x; item < many.total * p.rows_unit; item += gridDim.x) {
         const int which = item / p.rows_unit, row = item - which * p.rows_unit, c = find(many, which);
         const int4 head = p.parts[c];
         if (row >= min(p.rows_unit, p.group - head.w * p.rows_unit)) continue;
