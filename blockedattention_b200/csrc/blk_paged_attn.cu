@@ -2,14 +2,20 @@
 //
 //   s_j = scale q . k_j for the tokens j of a request,  m = max s_j,  l = sum exp(s_j - m),  out = sum exp(s_j - m) v_j / l
 //
-// All keys and values are read once and little is done with each, so the bytes bound it (2 x tokens x heads x d).  The work is one
-// list of tiles of 64 tokens, (request, key head, tile) in this order, which every block cuts into equal ranges by itself: it
-// adds up the lengths on the way in, so no length is ever read by the host.  A block's tiles arrive through a ring of
-// asynchronous 16-byte copies that runs on over the end of a request or head.  A warp owns 16 tokens of every tile and
-// the part of the ring they go through: within a head nothing but its own copies is waited for.  Where a head is done, the four
-// warps' maxima, sums and weighted values are put together; where it goes on in another block, they go to the workspace, and
-// a second kernel joins the parts of the heads that were cut (at most two parts a block, so the workspace does
-// not grow with the lengths).  No atomics: the same call gives the same bits.
+// All keys and values are read once and little is done with each, so the bytes bound it (2 x tokens x heads x d): 64 requests of
+// 1000..32000 tokens, 8 key heads of 128 under 64, bf16, 4.15 GB in 610 us (6.8 TB/s); one request of 999983 tokens 590 us.  What is short
+// is bounded by latencies instead: a request of 1000 tokens 7.1 us, of which 3.5 are the join and the way to it; 512 requests of 0..300
+// tokens, 8 heads of 64, fp16, 46.8 us (3.4 TB/s), where changing heads takes as long as their copies.
+// The work is one list of tiles of 64 tokens (32 in 32 bits beyond 64 columns), (request, key head, tile) in this order, which every
+// block cuts into ranges of equal cost by itself: it adds up the lengths on the way in, so no length is ever read by the host.  A
+// kernel of its own for that, with a join by whichever block comes last behind it, took longer (one request 10.6 us against 8.5 at the time).
+// A block's tiles arrive through a ring of asynchronous 16-byte copies that runs on over the end of a request or head.  A warp owns a
+// quarter of every tile and the part of the ring it goes through: within a head nothing but its own copies is waited for.  Warps
+// that copy for others, by such copies or through tensor maps, were no faster (long requests 610 us, 650 and 635; pages of 100 tokens
+// 346 through maps, whose boxes must not leave a page, 150 as it is).  Where a head is done, the four warps' maxima, sums and
+// weighted values are put together; where it goes on in another block, they go to the workspace, and a second kernel joins the parts of
+// the heads that were cut (at most two parts a block, so the workspace does not grow with the lengths).  No atomics: the same call
+// gives the same bits.
 #include <algorithm>
 
 #include "blk_device.cuh"
@@ -49,7 +55,8 @@ __device__ __forceinline__ int merge_at(int q, int col) { return q * DP + (col ^
 // Scores and values on the tensor cores with the tokens as the wide side: S^T = K Q^T is (16 tokens x 8 query rows), O^T = V^T P^T is
 // (d x 8 query rows), so the query heads that share a key head fill the narrow side and nothing is padded beyond eight.  P goes
 // from accumulator to operand by one 8 x 8 transposition in registers.  It enters as the sum of two 16-bit numbers: rounded once
-// it would add as much error as the rounding of the result does, and the second product costs no time next to the copies.
+// it would add as much error as the rounding of the result does.  The second product costs nothing next to the copies (long requests
+// 610 us, 607 without it), up to a tenth where 32 query rows share a key head (70.0, 64.1).
 // fp16 holds nothing below 2^-24: there P is 2^14 times as large, so that what it loses is below 2^-38 of the largest.
 // The first of the two is cut, not rounded, and the second never zero: both are positive, so that an infinite value stays one.
 template <typename Tag> struct PSplit;
@@ -495,17 +502,19 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     blk_grid_wait();
 
     // The lengths, added up: a run of requests for every thread, by each half of the block for itself.  A block's range is cut by cost: to change
-    // heads costs three quarters of a tile.  Tile t of a head begins at cost 0 for t = 0, else HEAD + TIME t, and belongs to the block whose range
-    // this lies in.  With less than a head of one tile for every block tiles alone count, so that none is empty.
+    // heads costs one and a quarter tiles (512 requests of 0..300 tokens 46.7 us; at a half 50.3, three quarters 47.6, two 47.7).  Tile t of a
+    // head begins at cost 0 for t = 0, else HEAD + TIME t, and belongs to the block whose range this lies in.  With less than a head of one tile for
+    // every block tiles alone count, so that none is empty.
     Walk cw{};
     int64_t each, over, blocks, first;  // range c: from cost c each + min(c, over) on; blocks that have one; this one's first tile
     int64_t count;
-    int TIME = 4, HEAD = 3;
+    int TIME = 4, HEAD = 5;
     {
         constexpr int HALF = THREADS / 2, HW = WARPS / 2;
         const int e = tid / HALF, ht = tid % HALF;  // the half finds the beginning (0) or the end (1) of the range
         const int per = (p.requests + HALF - 1) / HALF, r0 = min(ht * per, p.requests), r1 = min(r0 + per, p.requests);
         int64_t mine = 0;
+#pragma unroll 4
         for (int r = r0; r < r1; ++r) mine += tiles_of<TILE>(held(p, r));
         int64_t before = mine;
 #pragma unroll
@@ -583,7 +592,8 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     math.fetch(p, q_at(cw), rows_at(cw), lane);
 
     // Copies.  Where pages are whole numbers of a warp's tokens (one_page), these lie side by side on one page; else a lane looks up the page of one
-    // of them.  That is done two tiles before the rows are asked for; eight lanes take 128 bytes of a row.
+    // of them (page by page 140 us, 158 by tokens: 10 requests of 22273 tokens, 16 heads of 64; 69.6 and 87 for rows of 144 bytes; the longest
+    // of wide rows lose 1 % by it, 610 and 603).  That is done two tiles before the rows are asked for; eight lanes take 128 bytes of a row.
     Walk pw = cw;
     int entry = -1, soon = -1, n_here = 0, n_soon = 0;
     int64_t inner = 0, inner_soon = 0;
@@ -761,7 +771,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
 
 // Joins the parts of the heads that were cut.  Every warp looks through the blocks' notes for these heads.  Heads of few parts are rows for
 // warps, the others for blocks: a part for every warp, then the warps' results as parts again.  A part's statistics and values are asked
-// for together.
+// for together.  Few are eight: 32 requests of 16..4096 tokens 28.8 us, with four 29.9, with one 30.4.
 constexpr int JOIN_WARPS = 8, MAX_BLOCKS = 512, FEW = 8;
 template <int DP>
 struct Joined {
@@ -926,7 +936,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const B
     }
 }
 
-// The kernels: padded head dimension, query rows of a unit in eights, stages, blocks on an SM, rows put together at a time.
+// The kernels: padded head dimension, query rows of a unit in eights, stages, blocks on an SM, rows put together at a time.  A third block
+// is worth more than a third stage: 247 requests of 2470 tokens, 4 heads of 80, 160 us against 195; the long ones of 128 columns 616 and 635.
 template <typename Tag> struct Kernels16 {
     typedef Math16<Tag, 64, 1, 3, 3, 8> D64N1;
     typedef Math16<Tag, 64, 2, 3, 3, 16> D64N2;
@@ -973,7 +984,8 @@ auto with_kernel(int dtype, int DP, int rows, F f) {
 }  // namespace
 
 // Query rows that share a key head are taken together as far as registers hold their results; more of them are units of their
-// own, which read the keys again.
+// own, which read the keys again.  In 32 bits there are kernels for 2, 4 and 8 rows: 16 requests of 1..2000 tokens with two to a key head 18.9 us,
+// by the kernel for eight 24.3.
 BlkPagedShape blk_paged_shape(int dtype, int d, int group, int64_t requests, int64_t kv_heads, int64_t capacity, int sms) {
     BlkPagedShape s{};
     if (dtype == BLK_F32) s.DP = d <= 64 ? 64 : d <= 128 ? 128 : 256;

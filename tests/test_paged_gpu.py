@@ -81,22 +81,23 @@ def check(q, k, v, table, lengths, scale, got=None):
 LENGTHS = [0, 1, 15, 16, 17, 63, 64, 65, 100, 1000, 0, 2500, 31, 33, 128]
 
 
-@pytest.mark.parametrize("dtype,d", [(t, d) for t in (F16, BF16) for d in (8, 40, 64, 72, 128, 136, 256)] + [(F32, d) for d in (4, 20, 64, 100, 128, 200, 256)])
+@pytest.mark.parametrize("dtype,d", [(t, d) for t in (F16, BF16) for d in (8, 40, 64, 72, 96, 128, 136, 192, 200, 256)] + [(F32, d) for d in (4, 20, 64, 100, 128, 200, 256)])
 @pytest.mark.parametrize("kv,group,page,layout", [(1, 1, 16, "heads"), (3, 5, 24, "tokens"), (2, 8, 1, "heads"), (1, 17, 64, "tokens"), (2, 40, 100, "heads")])
 def test_attention(cuda_device, dtype, d, kv, group, page, layout):
     check(*make(LENGTHS, kv, group, d, page, dtype, d + kv, layout), d ** -0.5)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-@pytest.mark.parametrize("group", [1, 7, 8, 9, 16, 23, 24, 25, 32, 33])
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 7, 8, 9, 16, 23, 24, 25, 32, 33])
 def test_groups_of_query_heads(cuda_device, dtype, group):
     check(*make([300, 1, 90], 2, group, 64, 16, dtype, group), 0.125)
     check(*make([300, 1, 90], 2, group, 128, 16, dtype, group), 0.09)
+    check(*make([3000, 1, 90], 1, group, 256, 8, dtype, group), 0.06)
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
-@pytest.mark.parametrize("lengths", [[1], [64], [65], [20000], [150001, 3], [7] * 700, list(range(0, 1500)), [5000] * 40, [0] * 9, [0, 0, 40000, 0]])
-@pytest.mark.parametrize("page", [16, 48])
+@pytest.mark.parametrize("lengths", [[1], [64], [65], [20000], [150001, 3], [7] * 700, list(range(0, 1500)), [5000] * 40, [0] * 9, [0, 0, 40000, 0], [3, 0, 1, 2] * 1300])
+@pytest.mark.parametrize("page", [16, 20])
 def test_split_and_joined(cuda_device, dtype, lengths, page):
     check(*make(lengths, 2, 2, 64, page, dtype, len(lengths)), 0.125)
 
@@ -123,14 +124,15 @@ def test_pages_let_go_and_lengths_beyond_the_table(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype,d", [(F16, 64), (BF16, 72), (F32, 100)])
-def test_what_is_not_held_is_not_read(cuda_device, dtype, d):
+@pytest.mark.parametrize("page", [16, 24, 5])
+def test_what_is_not_held_is_not_read(cuda_device, dtype, d, page):
     lengths = [0, 1, 17, 40, 63, 65, 300, 1]
-    q, k, v, table, n = make(lengths, 2, 2, d, 16, dtype)
+    q, k, v, table, n = make(lengths, 2, 2, d, page, dtype)
     want = blockPagedAttention(q, k, v, table, n, 0.1)
-    held = torch.zeros(k.shape[0], 16, dtype=torch.bool)
+    held = torch.zeros(k.shape[0], page, dtype=torch.bool)
     for r, x in enumerate(lengths):
         for p in range(x):
-            held[int(table[r, p // 16]), p % 16] = True
+            held[int(table[r, p // page]), p % page] = True
     for bad in (math.nan, math.inf, -math.inf):
         for c in (k, v):
             c.transpose(1, 2)[~held.cuda()] = bad
@@ -285,6 +287,41 @@ def test_two_graphs_replayed_at_once(cuda_device):
     graphs[0].replay()
     torch.cuda.synchronize()
     check(q, k, v, table, n, 0.09, (outs[0], blockPagedAttention(q, k, v, table, n, 0.09, return_lse=True)[1]))
+
+
+def test_traced(cuda_device):
+    """A trace records the attention as one node whose tensors are its inputs; what writes in place or gives two results is refused."""
+    import warnings
+
+    q, k, v, table, n = make([300, 17], 2, 2, 64, 16, F16)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        traced = torch.jit.trace(lambda *a: blockPagedAttention(*a, 0.125) * 2, (q, k, v, table, n))
+        assert torch.equal(traced(q * 2, k, v, table, n - 5), blockPagedAttention(q * 2, k, v, table, n - 5, 0.125) * 2)
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(lambda q: blockPagedAttention(q, k, v, table, n, return_lse=True)[0], (q,))
+
+
+def test_calls_from_several_threads(cuda_device):
+    import threading
+
+    calls = [make([3000 + 100 * i, 17, 0], 2, 4, 64, 16, BF16, i) for i in range(4)]
+    wants = [blockPagedAttention(*c, 0.125) for c in calls]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not torch.equal(blockPagedAttention(*calls[i], 0.125), wants[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 # ---- slots -----------------------------------------------------------------------------------------------
