@@ -17,6 +17,7 @@
 // the heads that were cut (at most two parts a block, so the workspace does not grow with the lengths).  No atomics: the same call
 // gives the same bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "blk_device.cuh"
 #include "blk_kernels.h"
@@ -435,17 +436,19 @@ struct Lay {
     static_assert((BYTES + 1024) * M::CTAS <= 228 * 1024, "the blocks that a kernel is made for fit on an SM");
 };
 
-// Where a block is in the list of tiles: tile t of n, of part `part` of the query rows of key head `kv`, of request r.
+// Where a block is in the list of tiles: tile t of n, of part `part` of the query rows of key head `kv`, of request r; how many are left,
+// this one among them.  A warp by itself (see below): the same of its heads' quarter tiles, and the heads that are left.
 struct Walk {
     int r, kv, part, t, n, len, ahead;
+    int64_t left;
 };
 __device__ __forceinline__ int clipped(const BlkPagedAttnParams& p, int len) { return min(max(len, 0), p.capacity); }
 __device__ __forceinline__ int held(const BlkPagedAttnParams& p, int r) { return clipped(p, p.lengths[r]); }
 template <int TILE>
 __device__ __forceinline__ int tiles_of(int len) { return max(1, (int)(((unsigned)len + TILE - 1) / TILE)); }  // (an empty request's result is written, too)
+// To the next head.
 template <int TILE>
-__device__ __forceinline__ void step(Walk& w, const BlkPagedAttnParams& p) {
-    if (++w.t < w.n) return;
+__device__ __forceinline__ void next_head(Walk& w, const BlkPagedAttnParams& p) {
     w.t = 0;
     if (++w.part < p.q_units) return;
     w.part = 0;
@@ -455,6 +458,21 @@ __device__ __forceinline__ void step(Walk& w, const BlkPagedAttnParams& p) {
     w.len = clipped(p, w.ahead);
     w.n = tiles_of<TILE>(w.len);
     if (w.r + 1 < p.requests) w.ahead = p.lengths[w.r + 1];  // (as it is: to clip it now would wait for it)
+}
+// To the next tile; false: there is none.
+template <int TILE, int TW, bool ALONE>
+__device__ __forceinline__ bool step(Walk& w, const BlkPagedAttnParams& p) {
+    if (!ALONE) {
+        if (--w.left == 0) return false;
+        if (++w.t == w.n) next_head<TILE>(w, p);
+        return true;
+    }
+    if (++w.t < w.n) return true;
+    w.left -= WARPS;
+    if (w.left <= 0) return false;
+    for (int i = 0; i < WARPS; ++i) next_head<TILE>(w, p);
+    w.n = tiles_of<TW>(w.len);
+    return true;
 }
 
 template <typename Tag> struct Out;
@@ -507,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     // every block tiles alone count, so that none is empty.
     Walk cw{};
     int64_t each, over, blocks, first;  // range c: from cost c each + min(c, over) on; blocks that have one; this one's first tile
-    int64_t count;
+    bool by_warps;
     int TIME = 4, HEAD = 5;
     {
         constexpr int HALF = THREADS / 2, HW = WARPS / 2;
@@ -567,11 +585,21 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
             sched[10 + 8 * e] = len;
             sched[11 + 8 * e] = unit;
             sched[12 + 8 * e] = t;
+            sched[13 + 8 * e] = (int64_t)r * p.units + unit + (t == n);  // heads before, that of the first tile not among them
+            sched[14 + 8 * e] = t > 0 && t < n;
         }
-        if (tid == 0 && blockIdx.x + 1 == blocks) sched[16] = p.units * tiles;
+        if (tid == 0 && blockIdx.x + 1 == blocks) {
+            sched[16] = p.units * tiles;
+            sched[21] = (int64_t)p.requests * p.units;
+            sched[22] = 0;
+        }
         __syncthreads();
         first = sched[8];
-        count = sched[16] - first;
+        cw.left = sched[16] - first;
+        // Heads of a single tile each: every warp takes whole ones, in turn, and nothing is put together (495 requests of 5 tokens, 8 heads of 192,
+        // fp32, 36.7 -> 18.7 us; 503 of 1..16, 16 heads of 80, 62 -> 29).  Not with more than eight rows: these kernels lose 5 % where heads are longer
+        // for having both ways in them, the others 0 to 2 %.
+        by_warps = GU <= 8 && !sched[14] && !sched[22] && sched[21] - sched[13] == cw.left;
         cw.r = (int)sched[9];
         if (cw.r + 1 < p.requests) cw.ahead = p.lengths[cw.r + 1];
         cw.len = (int)sched[10];
@@ -580,193 +608,220 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         cw.kv = p.q_units == 1 ? unit : unit / p.q_units;
         cw.part = unit - cw.kv * p.q_units;
         cw.t = (int)sched[12];
-        if (cw.t == cw.n) {
-            cw.t -= 1;
-            step<TILE>(cw, p);
+        if (cw.t == cw.n) next_head<TILE>(cw, p);
+        if (by_warps) {
+            cw.left -= warp;
+            if (cw.left <= 0) return;  // (fewer heads than warps)
+            for (int i = 0; i < warp; ++i) next_head<TILE>(cw, p);
+            cw.n = tiles_of<TW>(cw.len);
         }
     }
 
-    M math;
-    auto q_at = [&](const Walk& w) { return p.q + w.r * p.q_row_stride + (int64_t)(w.kv * p.group + w.part * p.rows_unit) * p.q_head_stride; };
-    auto rows_at = [&](const Walk& w) { return min(p.rows_unit, p.group - w.part * p.rows_unit); };
-    math.fetch(p, q_at(cw), rows_at(cw), lane);
+    auto run = [&](auto kind) {
+        constexpr bool alone = decltype(kind)::value;
 
-    // Copies.  Where pages are whole numbers of a warp's tokens (one_page), these lie side by side on one page; else a lane looks up the page of one
-    // of them (page by page 140 us, 158 by tokens: 10 requests of 22273 tokens, 16 heads of 64; 69.6 and 87 for rows of 144 bytes; the longest
-    // of wide rows lose 1 % by it, 610 and 603).  That is done two tiles before the rows are asked for; eight lanes take 128 bytes of a row.
-    Walk pw = cw;
-    int entry = -1, soon = -1, n_here = 0, n_soon = 0;
-    int64_t inner = 0, inner_soon = 0;
-    auto look = [&]() {
-        const unsigned own = p.one_page ? 0 : lane, from = (unsigned)pw.t * TILE + warp * TW, tok = from + own;
-        n_soon = min(max((int)((unsigned)pw.len - from), 0), TW);
-        soon = -1;
-        if (tok < (unsigned)pw.len && own < TW) {
-            const unsigned col = (__umulhi(tok, p.page.magic) + tok) >> p.page.shift;
-            soon = p.table[pw.r * p.table_stride + col];
-            inner_soon = (int64_t)(tok - col * p.page.d) * p.token_stride + pw.kv * p.head_stride;
-        }
-    };
-    const int piece = lane & 7, row8 = lane >> 3;
-    auto load = [&](int stage) {
-        const bool there = entry >= 0 && entry < p.pages;
-        const uint32_t to = ring + stage * (2 * L::SIDE) + row8 * 128;
-        const uint32_t even = (piece ^ row8) << 4;  // (of rows 4 i + row8: swizzled by their number, so two places)
-        uint32_t mask;
-        if (p.one_page) {
-            mask = there ? (uint32_t)((1ull << n_here) - 1) : 0u;
-            if (mask) {
-                const int64_t off = entry * p.page_stride + inner + row8 * p.token_stride + piece * 16;
-                const char *k = p.k + off, *v = p.v + off;
-                if (n_here == TW) {
-#pragma unroll
-                    for (int i = 0; i < TW / 4; ++i) {
-#pragma unroll
-                        for (int j = 0; j < HALVES; ++j)
-                            if (piece + 8 * j < chunks) {
-                                cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), k + 128 * j);
-                                cp_async16(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), v + 128 * j);
-                            }
-                        k += 4 * p.token_stride;
-                        v += 4 * p.token_stride;
-                    }
-                } else {
-#pragma unroll 1
-                    for (int i = 0; i < TW / 4; ++i) {
-                        const bool have = i * 4 + row8 < n_here;  // (the last rows lie behind the request's end: not read)
-#pragma unroll
-                        for (int j = 0; j < HALVES; ++j)
-                            if (piece + 8 * j < chunks) {
-                                if (have) cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), k + 128 * j);
-                                cp_async16_or_zeros(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), have ? v + 128 * j : p.v, have);
-                            }
-                        k += 4 * p.token_stride;
-                        v += 4 * p.token_stride;
-                    }
-                }
+        auto meet = [&]() {
+            if (alone) __syncwarp();
+            else __syncthreads();
+        };
+        M math;
+        auto q_at = [&](const Walk& w) { return p.q + w.r * p.q_row_stride + (int64_t)(w.kv * p.group + w.part * p.rows_unit) * p.q_head_stride; };
+        auto rows_at = [&](const Walk& w) { return min(p.rows_unit, p.group - w.part * p.rows_unit); };
+        math.fetch(p, q_at(cw), rows_at(cw), lane);
+
+        // Copies.  Where pages are whole numbers of a warp's tokens (one_page), these lie side by side on one page; else a lane looks up the page of one
+        // of them (page by page 140 us, 158 by tokens: 10 requests of 22273 tokens, 16 heads of 64; 69.6 and 87 for rows of 144 bytes; the longest
+        // of wide rows lose 1 % by it, 610 and 603).  That is done two tiles before the rows are asked for; eight lanes take 128 bytes of a row.
+        Walk pw = cw;
+        int entry = -1, soon = -1, n_here = 0, n_soon = 0;
+        int64_t inner = 0, inner_soon = 0;
+        auto look = [&]() {
+            const unsigned own = p.one_page ? 0 : lane, from = alone ? (unsigned)pw.t * TW : (unsigned)pw.t * TILE + warp * TW, tok = from + own;
+            n_soon = min(max((int)((unsigned)pw.len - from), 0), TW);
+            soon = -1;
+            if (tok < (unsigned)pw.len && own < TW) {
+                const unsigned col = (__umulhi(tok, p.page.magic) + tok) >> p.page.shift;
+                soon = p.table[pw.r * p.table_stride + col];
+                inner_soon = (int64_t)(tok - col * p.page.d) * p.token_stride + pw.kv * p.head_stride;
             }
-        } else {
-            const int64_t off = there ? entry * p.page_stride + inner : -1;
-            mask = __ballot_sync(0xffffffffu, there);
-            if (mask) {
-#pragma unroll 2
-                for (int i = 0; i < TW / 4; ++i) {
-                    const int64_t o = __shfl_sync(0xffffffffu, off, i * 4 + row8);
-                    const bool have = o >= 0;
-                    const int64_t at = (have ? o : 0) + piece * 16;
+        };
+        const int piece = lane & 7, row8 = lane >> 3;
+        auto load = [&](int stage) {
+            const bool there = entry >= 0 && entry < p.pages;
+            const uint32_t to = ring + stage * (2 * L::SIDE) + row8 * 128;
+            const uint32_t even = (piece ^ row8) << 4;  // (of rows 4 i + row8: swizzled by their number, so two places)
+            uint32_t mask;
+            if (p.one_page) {
+                mask = there ? (uint32_t)((1ull << n_here) - 1) : 0u;
+                if (mask) {
+                    const int64_t off = entry * p.page_stride + inner + row8 * p.token_stride + piece * 16;
+                    const char *k = p.k + off, *v = p.v + off;
+                    if (n_here == TW) {
 #pragma unroll
-                    for (int j = 0; j < HALVES; ++j)
-                        if (piece + 8 * j < chunks) {
-                            if (have) cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), p.k + at + 128 * j);
-                            cp_async16_or_zeros(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), p.v + at + 128 * j, have);
+                        for (int i = 0; i < TW / 4; ++i) {
+#pragma unroll
+                            for (int j = 0; j < HALVES; ++j)
+                                if (piece + 8 * j < chunks) {
+                                    cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), k + 128 * j);
+                                    cp_async16(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), v + 128 * j);
+                                }
+                            k += 4 * p.token_stride;
+                            v += 4 * p.token_stride;
                         }
+                    } else {
+#pragma unroll 1
+                        for (int i = 0; i < TW / 4; ++i) {
+                            const bool have = i * 4 + row8 < n_here;  // (the last rows lie behind the request's end: not read)
+#pragma unroll
+                            for (int j = 0; j < HALVES; ++j)
+                                if (piece + 8 * j < chunks) {
+                                    if (have) cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), k + 128 * j);
+                                    cp_async16_or_zeros(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), have ? v + 128 * j : p.v, have);
+                                }
+                            k += 4 * p.token_stride;
+                            v += 4 * p.token_stride;
+                        }
+                    }
+                }
+            } else {
+                const int64_t off = there ? entry * p.page_stride + inner : -1;
+                mask = __ballot_sync(0xffffffffu, there);
+                if (mask) {
+#pragma unroll 2
+                    for (int i = 0; i < TW / 4; ++i) {
+                        const int64_t o = __shfl_sync(0xffffffffu, off, i * 4 + row8);
+                        const bool have = o >= 0;
+                        const int64_t at = (have ? o : 0) + piece * 16;
+#pragma unroll
+                        for (int j = 0; j < HALVES; ++j)
+                            if (piece + 8 * j < chunks) {
+                                if (have) cp_async16(to + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), p.k + at + 128 * j);
+                                cp_async16_or_zeros(to + L::SIDE + i * 512 + j * (TW * 128) + (even ^ (i & 1) << 6), p.v + at + 128 * j, have);
+                            }
+                    }
                 }
             }
-        }
-        // (a weight of zero must not meet what lies in a value's place: zeros are put there)
-        if (lane == 0) masks[stage] = mask;
-    };
-    int64_t loaded = 0;
-    int into = 0;
-    auto look_on = [&](int64_t i) {
-        entry = soon;
-        inner = inner_soon;
-        n_here = n_soon;
-        if (i < count) {
-            step<TILE>(pw, p);
-            if (pw.t == 0 && warp == 0 && lane < rows_at(pw)) {  // a new head: its queries are wanted soon
+            // (a weight of zero must not meet what lies in a value's place: zeros are put there)
+            if (lane == 0) masks[stage] = mask;
+        };
+        // tiles that are looked up and not asked for yet: 2, fewer at the end
+        int into = 0, ready = 1;
+        bool more_to_look = true;
+        auto look_on = [&]() {
+            if (!more_to_look) return;
+            more_to_look = step<TILE, TW, alone>(pw, p);
+            if (!more_to_look) return;
+            if (pw.t == 0 && (alone || warp == 0) && lane < rows_at(pw)) {  // a new head: its queries are wanted soon
                 const char* at = q_at(pw) + lane * p.q_head_stride;
                 for (int x = 0; x < p.d * M::E; x += 128) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(at + x));
             }
             look();
-        }
-    };
-    auto next = [&]() {
-        if (loaded < count) {
-            load(into);
-            into = into + 1 == STAGES ? 0 : into + 1;
-            ++loaded;
-            look_on(loaded + 1);
-        }
-        cp_commit();
-    };
-    look();
-    look_on(1);
+            ++ready;
+        };
+        auto take = [&]() {
+            entry = soon;
+            inner = inner_soon;
+            n_here = n_soon;
+        };
+        auto next = [&]() {
+            if (ready) {
+                load(into);
+                into = into + 1 == STAGES ? 0 : into + 1;
+                --ready;
+                take();
+                look_on();
+            }
+            cp_commit();
+        };
+        look();
+        take();
+        look_on();
 #pragma unroll 1
-    for (int s = 0; s < STAGES - 1; ++s) next();
+        for (int s = 0; s < STAGES - 1; ++s) next();
 
-    int stage = 0;
-    int4 part = make_int4(0, 0, 0, 0);
-    math.begin(extra);
-    for (int64_t i = 0; i < count; ++i) {
-        cp_wait<STAGES - 2>();
-        __syncwarp();
-        next();
-        const uint32_t mask = masks[stage];
-        if (mask) {
-            const uint32_t sK = ring + stage * (2 * L::SIDE);
-            math.tile(sK, sK + L::SIDE, mask, p.sign, p.c, extra, lane);
-        }
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
-        const bool ends = cw.t + 1 == cw.n, more = i + 1 < count;
-        const Walk now = cw;
-        if (more) step<TILE>(cw, p);
-        if (ends || !more) {
-            if (more) math.fetch(p, q_at(cw), rows_at(cw), lane);
-            const bool begins = i >= now.t;
-            const int rows = rows_at(now);
-            float* const ws = p.work + (2 * (int64_t)blockIdx.x + (begins ? 1 : 0)) * (GU * DP + 2 * GU);
-            const int64_t head0 = (int64_t)now.r * p.heads + now.kv * p.group + now.part * p.rows_unit;
+        int stage = 0;
+        int4 part = make_int4(0, 0, 0, 0);
+        math.begin(extra);
+        bool more = true;
+        for (int64_t i = 0; more; ++i) {
+            cp_wait<STAGES - 2>();
+            __syncwarp();
+            next();
+            const uint32_t mask = masks[stage];
+            if (mask) {
+                const uint32_t sK = ring + stage * (2 * L::SIDE);
+                math.tile(sK, sK + L::SIDE, mask, p.sign, p.c, extra, lane);
+            }
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            const bool ends = cw.t + 1 == cw.n;
+            const Walk now = cw;
+            more = step<TILE, TW, alone>(cw, p);
+            if (ends || !more) {
+                if (more) math.fetch(p, q_at(cw), rows_at(cw), lane);
+                const bool begins = alone || i >= now.t;
+                const int rows = rows_at(now);
+                float* const ws = p.work + (2 * (int64_t)blockIdx.x + (begins ? 1 : 0)) * (GU * DP + 2 * GU);
+                const int64_t head0 = (int64_t)now.r * p.heads + now.kv * p.group + now.part * p.rows_unit;
 #pragma unroll 1
-            for (int n = 0; n * PASS < rows; ++n) {
-                __syncthreads();  // (what was put here before is read)
-                if (n == 0) math.stats(sm_m + warp * GU, sm_l + warp * GU, lane);
-                if (math.seen) math.put(n, merge + warp * (PASS * DP), rows, lane);
-                __syncthreads();
-                const int here = min(PASS, rows - n * PASS);
-                for (int x = tid; x < here * (DP / 4); x += THREADS) {
-                    const int q = x / (DP / 4), col = x % (DP / 4) * 4, row = n * PASS + q;
-                    if (col >= p.d) continue;
-                    float top = sm_m[row], l = 0.f;
+                for (int n = 0; n * PASS < rows; ++n) {
+                    meet();  // (what was put here before is read)
+                    if (n == 0) math.stats(sm_m + warp * GU, sm_l + warp * GU, lane);
+                    if (math.seen) math.put(n, merge + warp * (PASS * DP), rows, lane);
+                    meet();
+                    const int here = min(PASS, rows - n * PASS);
+                    for (int x = alone ? lane : tid; x < here * (DP / 4); x += alone ? 32 : THREADS) {
+                        const int q = x / (DP / 4), col = x % (DP / 4) * 4, row = n * PASS + q;
+                        if (col >= p.d) continue;
+                        float top = -INFINITY, l = 0.f;
 #pragma unroll
-                    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w * GU + row]);
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int w = 0; w < WARPS; ++w)
+                            if (!alone || w == warp) top = fmaxf(top, sm_m[w * GU + row]);
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int w = 0; w < WARPS; ++w) {
-                        const float lw = sm_l[w * GU + row], f = part_weight(sm_m[w * GU + row], top, p.c);
-                        if (part_counts(lw, top)) {
-                            const float4 y = *reinterpret_cast<const float4*>(merge + w * (PASS * DP) + merge_at<DP>(q, col));
-                            l = fmaf(f, lw, l);
-                            v.x = fmaf(f, y.x, v.x);
-                            v.y = fmaf(f, y.y, v.y);
-                            v.z = fmaf(f, y.z, v.z);
-                            v.w = fmaf(f, y.w, v.w);
+                        for (int w = 0; w < WARPS; ++w) {
+                            if (alone && w != warp) continue;
+                            const float lw = sm_l[w * GU + row], f = part_weight(sm_m[w * GU + row], top, p.c);
+                            if (part_counts(lw, top)) {
+                                const float4 y = *reinterpret_cast<const float4*>(merge + w * (PASS * DP) + merge_at<DP>(q, col));
+                                l = fmaf(f, lw, l);
+                                v.x = fmaf(f, y.x, v.x);
+                                v.y = fmaf(f, y.y, v.y);
+                                v.z = fmaf(f, y.z, v.z);
+                                v.w = fmaf(f, y.w, v.w);
+                            }
                         }
-                    }
-                    if (begins && ends) {
-                        const int64_t head = head0 + row;
-                        Out<typename M::Tag>::put4(p.out, head * p.d + col, divided(v, l, M::OUT_SCALE));
-                        if (p.lse && col == 0) p.lse[head] = row_log(top, l, p.scale);
-                    } else {
-                        *reinterpret_cast<float4*>(ws + row * DP + col) = v;
-                        if (col == 0) {
-                            ws[GU * DP + row] = top;
-                            ws[GU * DP + GU + row] = l;
+                        if (begins && ends) {
+                            const int64_t head = head0 + row;
+                            Out<typename M::Tag>::put4(p.out, head * p.d + col, divided(v, l, M::OUT_SCALE));
+                            if (p.lse && col == 0) p.lse[head] = row_log(top, l, p.scale);
+                        } else {
+                            *reinterpret_cast<float4*>(ws + row * DP + col) = v;
+                            if (col == 0) {
+                                ws[GU * DP + row] = top;
+                                ws[GU * DP + GU + row] = l;
+                            }
                         }
                     }
                 }
+                if (begins && !ends) {  // the head goes on in the blocks up to the one that has its last tile
+                    const int64_t tile = first + i - now.t, head = (int64_t)now.r * p.units + now.kv * p.q_units + now.part;  // its first tile; heads before it
+                    const int64_t last = TIME * (tile + now.n - 1) + HEAD * (head + 1);  // (of two tiles or more)
+                    const int64_t wide = over * (each + 1), owner = last < wide ? quotient(last, each + 1) : over + quotient(last - wide, each);
+                    part = make_int4((int)owner - (int)blockIdx.x + 1, now.r, now.kv, now.part);
+                }
+                if (more) math.begin(extra);
             }
-            if (begins && !ends) {  // the head goes on in the blocks up to the one that has its last tile
-                const int64_t tile = first + i - now.t, head = (int64_t)now.r * p.units + now.kv * p.q_units + now.part;  // its first tile; heads before it
-                const int64_t last = TIME * (tile + now.n - 1) + HEAD * (head + 1);  // (of two tiles or more)
-                const int64_t wide = over * (each + 1), owner = last < wide ? quotient(last, each + 1) : over + quotient(last - wide, each);
-                part = make_int4((int)owner - (int)blockIdx.x + 1, now.r, now.kv, now.part);
-            }
-            if (more) math.begin(extra);
+        }
+        cp_wait<0>();
+        if (tid == 0) p.parts[blockIdx.x] = part;
+    };
+    if constexpr (GU <= 8) {
+        if (by_warps) {
+            run(std::true_type{});
+            return;
         }
     }
-    cp_wait<0>();
-    if (tid == 0) p.parts[blockIdx.x] = part;
+    run(std::false_type{});
 }
 
 // Joins the parts of the heads that were cut.  Every warp looks through the blocks' notes for these heads.  Heads of few parts are rows for

@@ -102,6 +102,17 @@ def test_split_and_joined(cuda_device, dtype, lengths, page):
     check(*make(lengths, 2, 2, 64, page, dtype, len(lengths)), 0.125)
 
 
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (BF16, 96), (BF16, 128), (F16, 192), (F16, 256), (F32, 64), (F32, 100), (F32, 256)])
+@pytest.mark.parametrize("group", [1, 2, 4, 7, 12])
+@pytest.mark.parametrize("page", [16, 6])
+def test_heads_of_one_tile(cuda_device, dtype, d, group, page):
+    """Batches in which nothing is longer than a tile, with and without one request that is; more and fewer of them than warps."""
+    short = list(range(33)) * 3 if dtype == F32 and d > 64 else list(range(65)) * 3
+    check(*make(short, 3, group, d, page, dtype, d), d ** -0.5)
+    check(*make(short + [65], 3, group, d, page, dtype, d), d ** -0.5)
+    check(*make([1, 0, 3], 1, group, d, page, dtype, d), d ** -0.5)
+
+
 def test_no_requests(cuda_device):
     q, k, v, table, lengths = make([5], 1, 2, 64, 16, F16)
     out, lse = blockPagedAttention(q[:0], k, v, table[:0], lengths[:0], return_lse=True)
