@@ -216,7 +216,7 @@ def blockPagedSlots(lengths: torch.Tensor, newTokens: torch.Tensor, pageTable: t
 def blockPagedAppend(k: torch.Tensor, v: torch.Tensor, kCache: torch.Tensor, vCache: torch.Tensor, slots: torch.Tensor) -> None:
     """Writes new keys and values to their slots of a paged cache, in place: ``k, v -> (tokens, heads, d)``, token-major as
     ``blockAttentionTokenMajor`` takes them, ``slots -> (tokens,)`` as ``blockPagedSlots`` gives them (no slot twice; those
-    outside the cache are passed over).  ``kCache, vCache -> (pages, heads, pageSize, d)`` of one shape and strides, rows
+    outside the cache are passed over).  The new rows must not lie in the cache itself.  ``kCache, vCache -> (pages, heads, pageSize, d)`` of one shape and strides, rows
     contiguous and 16-byte aligned; a cache kept as (pages, pageSize, heads, d) is given as its ``transpose(1, 2)``."""
     _ops.paged_append(k, v, kCache, vCache, slots)
 

@@ -992,14 +992,15 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const B
 }
 
 // The kernels: padded head dimension, query rows of a unit in eights, stages, blocks on an SM, rows put together at a time.  A third block
-// is worth more than a third stage: 247 requests of 2470 tokens, 4 heads of 80, 160 us against 195; the long ones of 128 columns 616 and 635.
+// is worth more than a third stage: 247 requests of 2470 tokens, 4 heads of 80, 160 us against 195; the long ones of 128 columns 616 and 635; 118 of 0..8225, one of 72
+// under 12, 65 against 69.  Where registers spill for it, as with 16 rows of 128 columns, it is 123 against 70.
 template <typename Tag> struct Kernels16 {
     typedef Math16<Tag, 64, 1, 3, 3, 8> D64N1;
     typedef Math16<Tag, 64, 2, 3, 3, 16> D64N2;
-    typedef Math16<Tag, 64, 3, 4, 2, 24> D64N3;
-    typedef Math16<Tag, 64, 4, 4, 2, 32> D64N4;
+    typedef Math16<Tag, 64, 3, 3, 2, 24> D64N3;
+    typedef Math16<Tag, 64, 4, 3, 2, 32> D64N4;
     typedef Math16<Tag, 96, 1, 2, 3, 4> D96N1;
-    typedef Math16<Tag, 96, 2, 2, 2, 16> D96N2;
+    typedef Math16<Tag, 96, 2, 2, 3, 4> D96N2;
     typedef Math16<Tag, 128, 1, 2, 3, 4> D128N1;
     typedef Math16<Tag, 128, 2, 3, 2, 8> D128N2;
     typedef Math16<Tag, 192, 1, 2, 2, 4> D192N1;

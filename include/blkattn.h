@@ -271,7 +271,7 @@ BLK_API int blk_paged_slots(const int32_t* lengths, const int32_t* new_tokens, i
 
 /* Row h of token i (k[i * k_row_stride + h * k_head_stride ...], v likewise; dev, 16-byte aligned rows of the cache's type) goes to
  * slot slots[i] (dev) of head h.  Slots outside [0, pages * page_size) are passed over.  No slot may be given twice (its row would
- * hold parts of both); rows of the cache must not overlap. */
+ * hold parts of both); rows of the cache must not overlap one another or the new ones. */
 BLK_API int blk_paged_append(const blk_paged_cache_t* cache, const void* k, int64_t k_row_stride, int64_t k_head_stride,
                              const void* v, int64_t v_row_stride, int64_t v_head_stride, const int64_t* slots, int64_t tokens,
                              void* cuda_stream);
