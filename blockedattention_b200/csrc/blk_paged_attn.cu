@@ -5,7 +5,7 @@
 // All keys and values are read once and little is done with each, so the bytes bound it (2 x tokens x heads x d): 64 requests of
 // 1000..32000 tokens, 8 key heads of 128 under 64, bf16, 4.15 GB in 610 us (6.8 TB/s); one request of 999983 tokens 590 us.  What is short
 // is bounded by latencies instead: a request of 1000 tokens 7.1 us, of which 3.5 are the join and the way to it; 512 requests of 0..300
-// tokens, 8 heads of 64, fp16, 46.8 us (3.4 TB/s), where changing heads takes as long as their copies.
+// tokens, 8 heads of 64, fp16, 47.7 us (3.4 TB/s), where changing heads takes as long as their copies.
 // The work is one list of tiles of 64 tokens (32 in 32 bits beyond 64 columns), (request, key head, tile) in this order, which every
 // block cuts into ranges of equal cost by itself: it adds up the lengths on the way in, so no length is ever read by the host.  A
 // kernel of its own for that, with a join by whichever block comes last behind it, took longer (one request 10.6 us against 8.5 at the time).
@@ -610,6 +610,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         cw.t = (int)sched[12];
         if (cw.t == cw.n) next_head<TILE>(cw, p);
         if (by_warps) {
+            __syncthreads();  // (no barrier comes after this, and what was read here lies where results are put together)
             cw.left -= warp;
             if (cw.left <= 0) return;  // (fewer heads than warps)
             for (int i = 0; i < warp; ++i) next_head<TILE>(cw, p);
@@ -619,7 +620,6 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
 
     auto run = [&](auto kind) {
         constexpr bool alone = decltype(kind)::value;
-
         auto meet = [&]() {
             if (alone) __syncwarp();
             else __syncthreads();
