@@ -495,7 +495,8 @@ __device__ __forceinline__ float4 divided(float4 v, float l, float scale) {
     const float inv = l == 0.f ? 0.f : l == INFINITY ? NAN : scale / l;
     return make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
 }
-__device__ __forceinline__ float row_log(float m, float l, float scale) { return l == 0.f ? -INFINITY : m * scale + logf(l); }
+// Its logarithm: that of no weight at all in both cases.
+__device__ __forceinline__ float row_log(float m, float l, float scale) { return l == 0.f || l == INFINITY ? -INFINITY : m * scale + logf(l); }
 
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (a | b) >> 32 ? a / b : (unsigned)a / (unsigned)b; }
 
