@@ -58,14 +58,16 @@ __device__ __forceinline__ int merge_at(int q, int col) { return q * DP + (col ^
 // from accumulator to operand by one 8 x 8 transposition in registers.  It enters as the sum of two 16-bit numbers: rounded once
 // it would add as much error as the rounding of the result does.  The second product costs nothing next to the copies (long requests
 // 610 us, 607 without it), up to a tenth where 32 query rows share a key head (70.0, 64.1).
-// fp16 holds nothing below 2^-24: there P is 2^14 times as large, so that what it loses is below 2^-38 of the largest.
-// The first of the two is cut, not rounded, and the second never zero: both are positive, so that an infinite value stays one.
+// fp16 holds nothing below 2^-24: there P is 2^14 times as large, so that a weight is off by 2^-39 of the largest at the most (and one
+// below that is zero).  The first of the two is cut, not rounded, and where it is not zero the second is not: both are positive
+// then, so that an infinite value stays one.  A weight of zero is two zeros: such tokens add nothing, however many they are.
+__device__ __forceinline__ float rest(float p, float first, float least) { return fmaxf(p - first, fminf(first, least)); }
 template <typename Tag> struct PSplit;
 template <> struct PSplit<BlkBf16Tag> {
     static constexpr float SCALE = 1.f;
     static __device__ __forceinline__ uint32_t hi(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
     static __device__ __forceinline__ uint32_t lo(float a, float b, uint32_t h) {
-        return BlkCvt<BlkBf16Tag>::pack2(fmaxf(a - __uint_as_float(h << 16), 1.17549435e-38f), fmaxf(b - __uint_as_float(h & 0xffff0000u), 1.17549435e-38f));
+        return BlkCvt<BlkBf16Tag>::pack2(rest(a, __uint_as_float(h << 16), 1.17549435e-38f), rest(b, __uint_as_float(h & 0xffff0000u), 1.17549435e-38f));
     }
 };
 template <> struct PSplit<BlkHalfTag> {
@@ -77,7 +79,7 @@ template <> struct PSplit<BlkHalfTag> {
     }
     static __device__ __forceinline__ uint32_t lo(float a, float b, uint32_t h) {
         const float2 r = __half22float2(*reinterpret_cast<__half2*>(&h));
-        return BlkCvt<BlkHalfTag>::pack2(fmaxf(a - r.x, 5.9604645e-8f), fmaxf(b - r.y, 5.9604645e-8f));
+        return BlkCvt<BlkHalfTag>::pack2(rest(a, r.x, 5.9604645e-8f), rest(b, r.y, 5.9604645e-8f));
     }
 };
 

@@ -26,3 +26,54 @@ def test_logarithm_of_scores_of_minus_infinity(cuda_device, dtype, d, group, n):
     k[table[0, 0].long(), 0, 1] = math.nan
     _, lse = blockPagedAttention(q, k, v, table, lengths, 0.125, return_lse=True)
     assert torch.isnan(lse[0]).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (BF16, 64), (F16, 128), (BF16, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("group", [1, 12])
+@pytest.mark.parametrize("n", [16, 700, 30000])
+@pytest.mark.parametrize("low", [-math.inf, -1000.0])
+def test_tokens_without_weight_add_nothing(cuda_device, dtype, d, group, n, low):
+    """One token of value zero among tokens whose weight is zero (a score of -inf, or e^-1000 of the largest, which no type here holds):
+    zero exactly, however large their values and however many they are."""
+    q, k, v, table, lengths = make([n], 1, group, d, 16, dtype)
+    q[:] = 1.0
+    k[:] = low / d
+    v[:] = 60000.0
+    page = table[0, n // 32].long()
+    k[page, 0, 5] = 0.0
+    v[page, 0, 5] = 0.0
+    out, lse = blockPagedAttention(q, k, v, table, lengths, 1.0, return_lse=True)
+    assert (out == 0).all() and (lse == 0).all()
+
+
+@pytest.mark.parametrize("dtype,weight", [(F16, 2.0 ** -37), (BF16, 2.0 ** -100)])
+def test_an_infinite_value_stays_one(cuda_device, dtype, weight):
+    """Infinite values of tokens with small weights, also weights that the first of the two 16-bit numbers holds exactly."""
+    for w in (weight, 2.0 ** -8, 0.7):
+        q, k, v, table, lengths = make([700], 1, 2, 64, 16, dtype)
+        q[:] = 0.0
+        q[:, :, 0] = 1.0
+        k[:] = 0.0
+        v[:] = 1.0
+        page = table[0, 20].long()
+        k[page, 0, 5, 0] = math.log(w)
+        v[page, 0, 5, 3], v[page, 0, 5, 4] = math.inf, -math.inf
+        out = blockPagedAttention(q, k, v, table, lengths, 1.0)
+        assert (out[..., 3] == math.inf).all() and (out[..., 4] == -math.inf).all()
+        assert torch.isfinite(out[..., 5:]).all()
+
+
+@pytest.mark.parametrize("group", [1, 12])
+def test_weights_too_small_for_halves_are_rounded(cuda_device, group):
+    """fp16: a weight is off by at most 2^-39 of the largest, in both directions: 30000 of 2^-40.4 do not count as more than they may."""
+    n = 30000
+    q, k, v, table, lengths = make([n], 1, group, 64, 16, F16)
+    q[:] = 1.0
+    k[:] = -28.0 / 64
+    v[:] = 60000.0
+    page = table[0, 900].long()
+    k[page, 0, 5] = 0.0
+    v[page, 0, 5] = 0.0
+    out = blockPagedAttention(q, k, v, table, lengths, 1.0).double()
+    want = (n - 1) * math.exp(-28.0) * 60000.0
+    assert ((out - want).abs() <= n * 2.0 ** -39 * 60000.0 + 2.0 ** -11 * want).all()
