@@ -64,16 +64,19 @@ def test_an_infinite_value_stays_one(cuda_device, dtype, weight):
 
 
 @pytest.mark.parametrize("group", [1, 12])
-def test_weights_too_small_for_halves_are_rounded(cuda_device, group):
-    """fp16: a weight is off by at most 2^-39 of the largest, in both directions: 30000 of 2^-40.4 do not count as more than they may."""
+@pytest.mark.parametrize("every", [False, True])
+def test_weights_too_small_for_halves_are_rounded(cuda_device, group, every):
+    """fp16: a weight is off by at most 2^-39 of the largest, in both directions: tokens of 2^-40.4 do not count as more than they may,
+    be it behind one large score or with one in every tile, which all of them are relative to."""
     n = 30000
     q, k, v, table, lengths = make([n], 1, group, 64, 16, F16)
     q[:] = 1.0
     k[:] = -28.0 / 64
     v[:] = 60000.0
-    page = table[0, 900].long()
-    k[page, 0, 5] = 0.0
-    v[page, 0, 5] = 0.0
+    large = table[0].long() if every else table[0, 900:901].long()
+    k[large, 0, 5] = 0.0
+    v[large, 0, 5] = 0.0
     out = blockPagedAttention(q, k, v, table, lengths, 1.0).double()
-    want = (n - 1) * math.exp(-28.0) * 60000.0
-    assert ((out - want).abs() <= n * 2.0 ** -39 * 60000.0 + 2.0 ** -11 * want).all()
+    small = (n - len(large)) / len(large)
+    want = small * math.exp(-28.0) * 60000.0
+    assert ((out - want).abs() <= (small + 1) * 2.0 ** -39 * 60000.0 + 2.0 ** -11 * want + 2.0 ** -25).all()
