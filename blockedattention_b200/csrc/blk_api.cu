@@ -1056,6 +1056,9 @@ int refused(const char* where, const char* what, int code = BLK_ERR_INVALID) {
 }
 int64_t bytes_of(int dtype) { return dtype == BLK_F32 ? 4 : 2; }
 
+// The kernels count requests in 32 bits, by blocks of up to 1024 threads: up to a block's threads beyond the last one.
+constexpr int64_t MOST_REQUESTS = 0x7fffffffLL - 1024;
+
 // Strides that no row uses (extents of one) are left out of every check.
 int check_paged_cache(const char* where, const blk_paged_cache_t* c) {
     if (!c) return refused(where, "no cache");
@@ -1103,7 +1106,8 @@ int check_paged_attention(const char* where, const blk_paged_cache_t* c, int64_t
     if (rc != BLK_OK) return rc;
     if (c->head_dim > 256) return refused(where, "head_dim must be at most 256", BLK_ERR_UNSUPPORTED);
     if (heads < 1 || heads % c->heads || heads > 0xffffLL) return refused(where, "the query heads must be a multiple of the cache's, at most 65535");
-    if (requests < 0 || requests > 0x7fffffffLL || columns < 0 || columns > 0x7fffffffLL) return refused(where, "requests and columns must be 0 to 2^31 - 1");
+    if (requests < 0 || requests > MOST_REQUESTS) return refused(where, "requests must be 0 to 2^31 - 1025");
+    if (columns < 0 || columns > 0x7fffffffLL) return refused(where, "columns must be 0 to 2^31 - 1");
     return BLK_OK;
 }
 int64_t capacity_of(const blk_paged_cache_t* c, int64_t columns) { return std::min<int64_t>(columns * c->page_size, 0x7fffffffLL); }
@@ -1117,7 +1121,7 @@ extern "C" int blk_paged_slots(const int32_t* lengths, const int32_t* new_tokens
                                void* cuda_stream) {
     static const char where[] = "blk_paged_slots";
     BlkRange range(where);
-    if (requests < 0 || requests > 0x7fffffffLL - 1024 || columns < 0 || columns > 0x7fffffffLL || num_free < 0 || tokens < 0)
+    if (requests < 0 || requests > MOST_REQUESTS || columns < 0 || columns > 0x7fffffffLL || num_free < 0 || tokens < 0)
         return refused(where, "negative or too large extent");
     if (page_size < 1 || page_size > (1LL << 30)) return refused(where, "the page size must be 1 to 2^30 tokens");
     if (requests > 1 && table_stride < columns) return refused(where, "rows of the page table overlap");

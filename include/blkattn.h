@@ -244,8 +244,8 @@ BLK_API int blk_softmax_noalloc(const void* src, void* out, const int64_t* rows,
  * of page g starts at element g * page_stride + h * head_stride + t * token_stride of k, and of v.  k, v: dev pointers,
  * 16-byte aligned; strides in elements, each row on a 16-byte boundary.  A request's tokens lie in the pages that its row of a page table
  * names: token p on place p % page_size of page table[p / page_size].  The calls below run on the current device, need no plan,
- * read no length or table on the host, neither allocate nor synchronise, and may be captured.  They have no
- * counterpart in the upstream project, which keeps nothing between calls. */
+ * read no length or table on the host, neither allocate nor synchronise, and may be captured; they take up to 2^31 - 1025 requests.
+ * They have no counterpart in the upstream project, which keeps nothing between calls. */
 typedef struct {
     void* k;
     void* v;

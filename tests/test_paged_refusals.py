@@ -99,3 +99,12 @@ def test_host_tensors():
                  lambda: blockPagedAttention(f.numpy(), c, c, t, i), lambda: blockPagedSlots(np.zeros(2, np.int32), i, t, i, i[:1], 16, 2)):
         with pytest.raises(RuntimeError, match="must be CUDA Tensor"):
             call()
+
+
+def test_attention_of_more_requests_than_its_indices_count():
+    """The kernels count requests in 32 bits, up to a block's threads beyond the last one: as many as blk_paged_slots takes."""
+    size = C.c_int64()
+    for requests in ((1 << 31) - 1, (1 << 31) - 1024):
+        assert attention(cache(), requests=requests) == L.BLK_ERR_INVALID
+        assert L.lib.blk_paged_attention_workspace(C.byref(cache()), 4, requests, 2, C.byref(size)) == L.BLK_ERR_INVALID
+        assert L.lib.blk_paged_slots(P, P, requests, P, 4, 4, P, 9, P, 16, P, 5, P, P, None) == L.BLK_ERR_INVALID
