@@ -75,7 +75,10 @@ def _traced(name, operands, args):
     if name == "softmax" and args[-1] is not None:   # in place or into a given tensor: nothing to record
         with _untraced():
             return _ops.softmax(*args)
-    return _Traced.apply(name, args[operands:], *args[:operands])
+    given = args[:operands]
+    if name == "paged_attention" and not torch.is_grad_enabled():   # refuses what requires a gradient, but not there
+        given = [t.detach() if t.requires_grad else t for t in given]
+    return _Traced.apply(name, args[operands:], *given)
 
 
 _ops.setup(_host_i64, L.BlkError, _traced)
@@ -217,7 +220,8 @@ def blockPagedAppend(k: torch.Tensor, v: torch.Tensor, kCache: torch.Tensor, vCa
     """Writes new keys and values to their slots of a paged cache, in place: ``k, v -> (tokens, heads, d)``, token-major as
     ``blockAttentionTokenMajor`` takes them, ``slots -> (tokens,)`` as ``blockPagedSlots`` gives them (no slot twice; those
     outside the cache are passed over).  The new rows must not lie in the cache itself.  ``kCache, vCache -> (pages, heads, pageSize, d)`` of one shape and strides, rows
-    contiguous and 16-byte aligned; a cache kept as (pages, pageSize, heads, d) is given as its ``transpose(1, 2)``."""
+    contiguous and 16-byte aligned; a cache kept as (pages, pageSize, heads, d) is given as its ``transpose(1, 2)``.  Forward
+    only: where gradients are recorded, a tensor that requires one is refused."""
     _ops.paged_append(k, v, kCache, vCache, slots)
 
 
@@ -232,7 +236,7 @@ def blockPagedAttention(q: torch.Tensor, kCache: torch.Tensor, vCache: torch.Ten
     bytes, pages of any size.  Tokens on a table entry that is no page (-1: let go of, as by a sliding window) take no part;
     a request without any gets zeros, a row whose scores are all -inf NaN.  ``return_lse``: ``(out, lse)`` with each row's natural
     logarithm of ``sum exp(scale * q K^T)`` (-inf in both cases), which is what joins the result with attention over other keys.
-    Forward only."""
+    Forward only: where gradients are recorded, a tensor that requires one is refused."""
     run = _ops.paged_attention_lse if return_lse else _ops.paged_attention
     return run(q, kCache, vCache, pageTable, lengths, scale)
 

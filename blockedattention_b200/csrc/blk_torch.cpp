@@ -911,6 +911,12 @@ void written(const char* name, const Tensor& t) {
     torch::autograd::impl::bump_version(t);
 }
 
+// No backward pass and no forward-mode derivative here: a gradient is refused, not dropped.
+void forward_only(const char* name, const Tensor& t) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name, " requires a gradient, and the paged cache's operators are forward only (torch.no_grad() or a detached tensor)");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "the paged cache's operators have no forward-mode derivative");
+}
+
 blk_paged_cache_t cache_of(const Tensor& k, const Tensor& v) {
     TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == v.device(),
                 "kCache and vCache must both have shape (pages, heads, pageSize, d), one type and one device");
@@ -973,6 +979,8 @@ PyObject* py_paged_append(PyObject* const* a) {
     TORCH_CHECK(k.scalar_type() == kc.scalar_type() && v.scalar_type() == kc.scalar_type() && k.device() == dev && v.device() == dev,
                 "k and v must have the cache's type and device");
     TORCH_CHECK(c.head_dim <= 1 || (k.stride(2) == 1 && v.stride(2) == 1), "k and v must be contiguous along d");
+    forward_only("k", k);
+    forward_only("v", v);
     {
         const NoGil free;
         c10::cuda::CUDAGuard guard(dev);
@@ -994,6 +1002,9 @@ Tensor paged_attention(PyObject* const* a, Tensor* lse) {
     TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim && (c.head_dim <= 1 || q.stride(2) == 1), "q must have shape (requests, heads, d), d that of the cache, contiguous along d");
     const int64_t B = q.size(0), H = q.size(1);
     TORCH_CHECK(lengths.numel() == B && table.size(0) == B, "lengths and pageTable must have one entry or row for each request");
+    forward_only("q", q);
+    forward_only("kCache", kc);
+    forward_only("vCache", vc);
     const NoGil free;
     c10::cuda::CUDAGuard guard(dev);
     const int64_t s[3] = {B, H, c.head_dim};
