@@ -234,8 +234,8 @@ def blockPagedAttention(q: torch.Tensor, kCache: torch.Tensor, vCache: torch.Ten
     ``kCache, vCache -> (pages, cache heads, pageSize, d)`` as for ``blockPagedAppend``; ``heads`` is a multiple of the cache's, and
     that many consecutive heads of q share a head of the cache.  fp16, bf16 or fp32, ``d`` up to 256 in rows of whole 16
     bytes, pages of any size.  Tokens on a table entry that is no page (-1: let go of, as by a sliding window) take no part;
-    a request without any gets zeros, a row whose scores are all -inf NaN.  ``return_lse``: ``(out, lse)`` with each row's natural
-    logarithm of ``sum exp(scale * q K^T)`` (-inf in both cases), which is what joins the result with attention over other keys.
+    a request without any gets zeros, a row whose scores are all -inf, or one +inf, NaN.  ``return_lse``: ``(out, lse)`` with each
+    row's natural logarithm of ``sum exp(scale * q K^T)`` (-inf, -inf and +inf there), which is what joins the result with attention over other keys.
     Forward only: where gradients are recorded, a tensor that requires one is refused."""
     run = _ops.paged_attention_lse if return_lse else _ops.paged_attention
     return run(q, kCache, vCache, pageTable, lengths, scale)

@@ -43,9 +43,11 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
 }
-// A part of a row: maximum m and sum l of its weights relative to m.  l = 0: it saw no token, and its values are not there.
-// l = inf, m = -inf: it saw scores of -inf alone, which count only where every part is like that (0 / 0).  A NaN in l is kept.
-__device__ __forceinline__ bool part_counts(float l, float top) { return l != 0.f && !(l == INFINITY && top > -INFINITY); }
+// A part of a row: maximum m (the largest finite number at the most) and sum l of its weights relative to m.  l = 0: it saw no token, and its
+// values are not there.  l = inf, m = -inf: it saw scores of -inf alone, which count only where every part is like that (0 / 0).  l = inf
+// and another m: it saw a score of inf (inf / inf, and a logarithm of inf).  A NaN in l is kept.
+constexpr float MOST = 3.40282347e38f;
+__device__ __forceinline__ bool part_counts(float m, float l, float top) { return l != 0.f && !(l == INFINITY && m < top); }
 __device__ __forceinline__ float part_weight(float m, float top, float c) { return m == -INFINITY ? 1.f : blk_exp2((m - top) * c); }
 
 // Place of a column of row q among rows of DP floats: rows two apart lie eight banks apart, as a warp's accumulators are spread.
@@ -158,7 +160,7 @@ struct Math16 {
                 t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
                 t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
                 t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-                const float top = fmaxf(m[n][e], t), ref = top == -INFINITY ? 0.f : top;
+                const float top = fminf(fmaxf(m[n][e], t), MOST), ref = top == -INFINITY ? 0.f : top;
                 alpha[n][e] = blk_exp2((m[n][e] - ref) * c);
                 grew |= top > m[n][e];
                 m[n][e] = top;
@@ -350,7 +352,7 @@ struct Math32 {
 #pragma unroll
         for (int x = 1; x < 32; x *= 2)
             if (of_token(x)) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        top = fmaxf(top, m);
+        top = fmaxf(fminf(top, MOST), m);
         const float ref = top == -INFINITY ? 0.f : top, alpha = blk_exp2((m - ref) * scale);
         const bool grew = __any_sync(0xffffffffu, top > m);
         m = top;
@@ -492,13 +494,13 @@ template <> struct Out<BlkFloatTag> {
     static __device__ __forceinline__ void put4(void* out, int64_t at, float4 v) { *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v; }
 };
 
-// Result of a head's row from its sum and weighted values.  No token at all: l = 0 and zeros; scores of -inf alone: l = inf and NaN.
+// Result of a head's row from its sum and weighted values.  No token at all: l = 0 and zeros; scores of -inf alone, or one of inf: l = inf and NaN.
 __device__ __forceinline__ float4 divided(float4 v, float l, float scale) {
     const float inv = l == 0.f ? 0.f : l == INFINITY ? NAN : scale / l;
     return make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
 }
-// Its logarithm: that of no weight at all in both cases.
-__device__ __forceinline__ float row_log(float m, float l, float scale) { return l == 0.f || l == INFINITY ? -INFINITY : m * scale + logf(l); }
+// Its logarithm: that of no weight at all in the first two cases.
+__device__ __forceinline__ float row_log(float m, float l, float scale) { return l == 0.f || (l == INFINITY && m == -INFINITY) ? -INFINITY : m * scale + logf(l); }
 
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) { return (a | b) >> 32 ? a / b : (unsigned)a / (unsigned)b; }
 
@@ -784,7 +786,7 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
                         for (int w = 0; w < WARPS; ++w) {
                             if (alone && w != warp) continue;
                             const float lw = sm_l[w * GU + row], f = part_weight(sm_m[w * GU + row], top, p.c);
-                            if (part_counts(lw, top)) {
+                            if (part_counts(sm_m[w * GU + row], lw, top)) {
                                 const float4 y = *reinterpret_cast<const float4*>(merge + w * (PASS * DP) + merge_at<DP>(q, col));
                                 l = fmaf(f, lw, l);
                                 v.x = fmaf(f, y.x, v.x);
@@ -862,7 +864,7 @@ struct Joined {
         float up = top;
 #pragma unroll
         for (int j = 0; j < N; ++j) up = fmaxf(up, m[j]);
-        const bool before = part_counts(sum, up);
+        const bool before = part_counts(top, sum, up);
         const float old = part_weight(top, up, p.c);
         sum = before ? sum * old : 0.f;
 #pragma unroll
@@ -870,7 +872,7 @@ struct Joined {
         top = up;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            if (!part_counts(l[j], up)) continue;  // (the same for the whole warp)
+            if (!part_counts(m[j], l[j], up)) continue;  // (the same for the whole warp)
             const float f = part_weight(m[j], up, p.c);
             sum = fmaf(f, l[j], sum);
 #pragma unroll
@@ -974,7 +976,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) blk_paged_join_kernel(const B
             sum.begin();
 #pragma unroll
             for (int k = 0; k < JOIN_WARPS; ++k) {
-                if (!part_counts(stats[k][1], top)) continue;
+                if (!part_counts(stats[k][0], stats[k][1], top)) continue;
                 const float f = part_weight(stats[k][0], top, p.c);
                 l = fmaf(f, stats[k][1], l);
 #pragma unroll

@@ -278,11 +278,12 @@ BLK_API int blk_paged_append(const blk_paged_cache_t* cache, const void* k, int6
 
 /* out[r, h] = softmax(scale * q[r, h] K^T) V over the tokens that request r keeps of head h / (heads / cache heads): the first
  * lengths[r] (no more than columns * page_size) but for those whose page_table entry is no page (negative, or
- * >= pages).  A request without tokens gets zeros; a row whose scores are all -inf gets NaN (0 / 0).  q: (requests, heads, head_dim)
- * with the given strides in elements, rows on 16-byte boundaries; out: the same, packed; lse: natural logarithm of each row's
- * softmax denominator, scale and maximum included (requests x heads floats, -inf without tokens or where every score is -inf), or NULL.  head_dim at most 256; heads a
- * multiple of the cache's.  workspace: dev, 16-byte aligned, at least what blk_paged_attention_workspace says for the same arguments on
- * the same device; calls that may overlap need one each. */
+ * >= pages).  A request without tokens gets zeros; a row whose scores are all -inf, or one +inf, gets NaN (0 / 0, inf / inf).
+ * q: (requests, heads, head_dim) with the given strides in elements, rows on 16-byte boundaries; out: the same, packed; lse:
+ * natural logarithm of each row's softmax denominator, scale and maximum included (requests x heads floats; -inf without tokens or
+ * where every score is -inf, +inf where one is), or NULL.  head_dim at most 256; heads a multiple of the cache's.  workspace: dev,
+ * 16-byte aligned, at least what blk_paged_attention_workspace says for the same arguments on the same device; calls that may
+ * overlap need one each. */
 BLK_API int blk_paged_attention_workspace(const blk_paged_cache_t* cache, int64_t heads, int64_t requests, int64_t columns,
                                           int64_t* bytes);
 BLK_API int blk_paged_attention(const blk_paged_cache_t* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,

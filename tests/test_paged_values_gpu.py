@@ -80,3 +80,23 @@ def test_weights_too_small_for_halves_are_rounded(cuda_device, group, every):
     small = (n - len(large)) / len(large)
     want = small * math.exp(-28.0) * 60000.0
     assert ((out - want).abs() <= (small + 1) * 2.0 ** -39 * 60000.0 + 2.0 ** -11 * want + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (BF16, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("group", [1, 4, 12])
+@pytest.mark.parametrize("n", [3, 40, 700, 30000])
+def test_logarithm_of_a_score_of_infinity(cuda_device, dtype, d, group, n):
+    """ln sum exp with a score of +inf is +inf (the softmax is inf / inf: NaN), wherever the others stand, above or below zero; a NaN
+    among them stays one."""
+    q, k, v, table, lengths = make([n] * 4, 1, group, d, 16, dtype)
+    q[:] = 8.0
+    k[table[:, : -(-n // 16)].long()] = 3.0
+    k[table[1].long()] = -3.0
+    last = (table[:, (n - 1) // 16].long(), 0, (n - 1) % 16)
+    k[last[0][:2], 0, last[2]] = math.inf
+    k[table[2, 0].long(), 0, 0] = math.inf
+    k[last[0][2], 0, last[2]] = -math.inf
+    k[table[3, 0].long(), 0, 1] = math.inf
+    k[table[3, 0].long(), 0, 2] = math.nan
+    out, lse = blockPagedAttention(q, k, v, table, lengths, 1.0, return_lse=True)
+    assert (lse[:3] == math.inf).all() and torch.isnan(lse[3]).all() and torch.isnan(out).all()
