@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from blockedattention_b200 import blockPagedAttention
-from test_paged_gpu import BF16, F16, F32, ints, make
+from test_paged_gpu import BF16, F16, F32, check, ints, make
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,80 @@ def test_logarithm_of_a_score_of_infinity(cuda_device, dtype, d, group, n):
     k[table[3, 0].long(), 0, 2] = math.nan
     out, lse = blockPagedAttention(q, k, v, table, lengths, 1.0, return_lse=True)
     assert (lse[:3] == math.inf).all() and torch.isnan(lse[3]).all() and torch.isnan(out).all()
+
+
+def windowed(window, lengths, kv, group, d, page, dtype, seed=0):
+    """Long requests whose pages in front of the last ones are let go of, and what these hold on their own."""
+    q, k, v, table, n = make(lengths, kv, group, d, page, dtype, seed)
+    for r, x in enumerate(lengths):
+        table[r, : max(0, x - window) // page] = -1
+    held = [x - max(0, x - window) // page * page for x in lengths]
+    only = torch.full((len(lengths), -(-max(held) // page)), -1, dtype=torch.int32, device="cuda")
+    for r, (x, y) in enumerate(zip(lengths, held)):
+        only[r, : -(-y // page)] = table[r, (x - y) // page: -(-x // page)]
+    return q, k, v, table, n, only, ints(held)
+
+
+@pytest.mark.parametrize("dtype,d,group", [(F16, 64, 1), (BF16, 128, 4), (BF16, 64, 24), (F32, 80, 2)])
+@pytest.mark.parametrize("page", [16, 24, 64])
+@pytest.mark.parametrize("window", [1, 100, 4096])
+def test_windows_that_begin_deep_in_long_requests(cuda_device, dtype, d, group, page, window):
+    """Thousands of pages let go of: as the pages that are left give alone, to the tolerance of test_paged_gpu's check()."""
+    q, k, v, table, n, only, held = windowed(window, [100000, 31, 57003, 0, 4096, 99991], 2, group, d, page, dtype)
+    got = blockPagedAttention(q, k, v, table, n, d ** -0.5, return_lse=True)
+    check(q, k, v, only, held, d ** -0.5, got)
+    assert (got[0][3] == 0).all() and torch.equal(blockPagedAttention(q, k, v, table, n, d ** -0.5), got[0])
+
+
+def test_logarithms_of_replays(cuda_device):
+    """A captured call that gives logarithms, replayed with other queries, lengths and pages."""
+    q, k, v, table, n = make([3000, 17, 0, 9000], 2, 4, 128, 16, BF16)
+    blockPagedAttention(q, k, v, table, n, 0.09, return_lse=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = blockPagedAttention(q, k, v, table, n, 0.09, return_lse=True)
+    for seed in range(3):
+        now = make([[3000, 17, 0, 9000], [1, 8999, 64, 0], [65, 0, 2000, 4000]][seed], 2, 4, 128, 16, BF16, seed, columns=table.shape[1], spare=3)
+        q.copy_(now[0])
+        n.copy_(now[4])
+        table.copy_(now[3].remainder(k.shape[0]))
+        out.fill_(7), lse.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(q, k, v, table, n, 0.09, (out, lse))
+
+
+def test_a_workspace_that_is_too_small(cuda_device):
+    """The C entry refuses it on the host; with what it asks for, the call runs."""
+    import ctypes as C
+
+    from blockedattention_b200 import _lib as L
+    q, k, v, table, n = make([300, 17], 2, 2, 64, 16, F16)
+    want = blockPagedAttention(q, k, v, table, n, 0.125)
+    cache = L.PagedCache(k.data_ptr(), v.data_ptr(), *(k.shape[i] for i in (0, 2, 1, 3)), k.stride(0), k.stride(1), k.stride(2), L.BLK_F16)
+    size = C.c_int64()
+    assert L.lib.blk_paged_attention_workspace(C.byref(cache), 4, 2, table.shape[1], C.byref(size)) == L.BLK_OK and size.value > 0
+    work, out = torch.empty(size.value, dtype=torch.uint8, device="cuda"), torch.zeros_like(q)
+    for room, code in ((size.value - 1, L.BLK_ERR_INVALID), (0, L.BLK_ERR_INVALID), (size.value, L.BLK_OK)):
+        assert L.lib.blk_paged_attention(C.byref(cache), q.data_ptr(), q.stride(0), q.stride(1), 4, table.data_ptr(), table.stride(0), table.shape[1],
+                                         n.data_ptr(), 2, 0.125, out.data_ptr(), None, work.data_ptr(), room,
+                                         torch.cuda.current_stream().cuda_stream) == code
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) if code == L.BLK_OK else (out == 0).all()
+
+
+def test_threads_give_what_one_call_gives(cuda_device):
+    """Calls from several threads on streams of their own: every one is compared, and an error in a thread is one here."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    calls = [make([3000 + 100 * i, 17, 0], 2, 4, 64, 16, BF16, i) for i in range(4)]
+    wants = [blockPagedAttention(*c, 0.125) for c in calls]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            return sum(torch.equal(blockPagedAttention(*calls[i], 0.125), wants[i]) for _ in range(30))
+
+    with ThreadPoolExecutor(4) as pool:
+        assert list(pool.map(work, range(4))) == [30] * 4
