@@ -260,7 +260,8 @@ cudaError_t blk_launch_scores_pipe(const BlkPackParams& p, int dtype_in, int sms
 cudaError_t blk_launch_softmax(const BlkSmxParams& p, int dtype, cudaStream_t st);
 
 // ---- paged cache (blk_paged.cu, blk_paged_attn.cu) ------------------------------------------------------
-// A number divided by the same one over and over: n / d = (mulhi(n, magic) + n) >> shift for n < 2^31, 1 <= d <= 2^30.
+// A number divided by the same one over and over, by a product and a shift (Granlund and Montgomery, Division by Invariant Integers using
+// Multiplication, 1994): n / d = (mulhi(n, magic) + n) >> shift for n < 2^31, 1 <= d <= 2^30.
 struct BlkDivisor {
     uint32_t d, magic, shift;
 };

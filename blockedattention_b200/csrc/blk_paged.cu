@@ -13,7 +13,7 @@ __device__ __forceinline__ unsigned divide(unsigned n, const BlkDivisor& d) { re
 // a time as it has threads, and writes an equal share of the tokens' slots; the token on the first place of a new page writes the table's entry.
 // Tokens beyond the last slot are not gone through one by one (their number is whatever the counts say, up to 2^31 a request): the pages of
 // such a call are written by their own numbers, so that it takes no longer than its slots and its table are long.
-// Latency bounds it: a step of 64 requests 2.6 us (2.0 is an empty launch), prompts of 1.2 million tokens 9.1 (10 MB).
+// Latency bounds it: a step of 64 requests 2.7 us (2.0 is an empty launch), prompts of 1.2 million tokens 9.2 (10 MB).
 
 struct Request {
     int old_tokens, new_tokens;
@@ -213,8 +213,12 @@ __global__ void __launch_bounds__(APPEND_THREADS) blk_paged_append_kernel(const 
 }  // namespace
 
 // One block does it all for a step's few tokens: no other block's sums to repeat, and a call in place needs no second launch.  It is a small one for
-// requests and tokens of a step: 64 requests of a token each 2.6 us, by 1024 threads 3.5; 600 requests, which the small one would take in
-// three turns, 1.2 million tokens by blocks of 1024 threads 9.1, of 256 15.0.
+// requests and tokens of a step (small and large, us): 64 requests of a token each 2.7 and 3.6, 256 2.9 and 3.8; 64 requests with 512 tokens 3.7 and
+// 3.8, with 1000 5.4 and 3.7, where the large one would be the better already; 300 requests, two turns of the small one, 4.5 and 3.9, 1000
+// 8.2 and 4.5.  600 requests, 1.2 million tokens: by blocks of 1024 threads 9.1, of 256 15.0.
+// More blocks from 8192 tokens on.  A smaller share is faster where one block is the bound: shares of 1024, 2048, 4096 and 8192 take 4.1, 5.5, 7.9 and
+// 12.6 us for 600 requests with 40000 tokens, 3.9, 5.0, 7.3 and 7.3 for 100 with 4000, and 8.5 all of them for 1.2 million.  In place, where a second
+// block brings a second launch, the first two take 0.3 to 1.9 us more where one block would do (1 request with 4000 tokens, 4096 with one each).
 cudaError_t blk_launch_paged_slots(const BlkPagedSlotsParams& p_in, int sms, cudaStream_t st) {
     BlkPagedSlotsParams p = p_in;
     if (p.requests <= SOME && p.tokens <= 4 * SOME) return blk_launch(true, blk_paged_slots_kernel<SOME>, dim3(1), dim3(SOME), (size_t)0, st, p);

@@ -3,11 +3,15 @@
 //   s_j = scale q . k_j for the tokens j of a request,  m = max s_j,  l = sum exp(s_j - m),  out = sum exp(s_j - m) v_j / l
 //
 // All keys and values are read once and little is done with each, so the bytes bound it (2 x tokens x heads x d): 64 requests of
-// 1000..32000 tokens, 8 key heads of 128 under 64, bf16, 4.15 GB in 610 us (6.8 TB/s); one request of 999983 tokens 590 us.  What is short
-// is bounded by latencies instead: a request of 1000 tokens 7.1 us, of which 3.5 are the join and the way to it; 512 requests of 0..300
-// tokens, 8 heads of 64, fp16, 47.7 us (3.4 TB/s), where changing heads takes as long as their copies.
+// 1000..32000 tokens, 8 key heads of 128 under 64, bf16, 4.15 GB in 611 us (6.8 TB/s); one request of 999983 tokens 589 us.  What is short
+// is bounded by latencies instead: a request of 1000 tokens 7.2 us, of which 3.5 are the join and the way to it; 512 requests of 0..300
+// tokens, 8 heads of 64, fp16, 48.0 us (3.3 TB/s), where changing heads takes as long as their copies.  Many query rows to a key head are bounded by
+// their products and by what is read again: 40 requests of 100..8000, 4 key heads of 64 under 128, bf16, 68.5 us (29 for the bytes); 80 of 2795, 3
+// of 256 under 96, fp32, 980 (212).
 // The work is one list of tiles of 64 tokens (32 in 32 bits beyond 64 columns), (request, key head, tile) in this order, which every
-// block cuts into ranges of equal cost by itself: it adds up the lengths on the way in, so no length is ever read by the host.  A
+// block cuts into ranges of equal cost by itself: it adds up the lengths on the way in, so no length is ever read by the host.  That is
+// right for hundreds of requests; beyond a few thousand it is most of the call (of ten tokens each, 8 heads of 64: 2000 requests 20 us, 8000 47,
+// 32000 213, where the bytes take 2, 7 and 28).  A
 // kernel of its own for that, with a join by whichever block comes last behind it, took longer (one request 10.6 us against 8.5 at the time).
 // A block's tiles arrive through a ring of asynchronous 16-byte copies that runs on over the end of a request or head.  A warp owns a
 // quarter of every tile and the part of the ring it goes through: within a head nothing but its own copies is waited for.  Warps
@@ -58,8 +62,10 @@ __device__ __forceinline__ int merge_at(int q, int col) { return q * DP + (col ^
 // Scores and values on the tensor cores with the tokens as the wide side: S^T = K Q^T is (16 tokens x 8 query rows), O^T = V^T P^T is
 // (d x 8 query rows), so the query heads that share a key head fill the narrow side and nothing is padded beyond eight.  P goes
 // from accumulator to operand by one 8 x 8 transposition in registers.  It enters as the sum of two 16-bit numbers: rounded once
-// it would add as much error as the rounding of the result does.  The second product costs nothing next to the copies (long requests
-// 610 us, 607 without it), up to a tenth where 32 query rows share a key head (70.0, 64.1).
+// it would add as much error as the rounding of the result does.  It holds 16 to 17 bits of a weight in bf16, 22
+// in fp16: some roundings of results fall otherwise than after products in 32 bits, and none is further from the exact result than half a step
+// and this.  The second product costs little next to the copies (long requests 611 us, 608 without it; 512 of 0..300 tokens 48.0, 46.3), up to a tenth
+// where 32 query rows share a key head (68.5, 62.5).
 // fp16 holds nothing below 2^-24: there P is 2^14 times as large, so that a weight is off by 2^-39 of the largest at the most (and one
 // below that is zero).  The first of the two is cut, not rounded, and where it is not zero the second is not: both are positive
 // then, so that an infinite value stays one.  A weight of zero is two zeros: such tokens add nothing, however many they are.
@@ -525,7 +531,8 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
     blk_grid_wait();
 
     // The lengths, added up: a run of requests for every thread, by each half of the block for itself.  A block's range is cut by cost: to change
-    // heads costs one and a quarter tiles (512 requests of 0..300 tokens 46.7 us; at a half 50.3, three quarters 47.6, two 47.7).  Tile t of a
+    // heads costs one and a quarter tiles (512 requests of 0..300 tokens 48.0 us; at a half 50.1, three quarters 48.7, two 48.4; 40 of 100..4000, 8 rows of 256
+    // columns, fp32, 160.6; 164.8, 161.1, 157.9).  Tile t of a
     // head begins at cost 0 for t = 0, else HEAD + TIME t, and belongs to the block whose range this lies in.  With less than a head of one tile for
     // every block tiles alone count, so that none is empty.
     Walk cw{};
@@ -602,8 +609,9 @@ __global__ void __launch_bounds__(THREADS, M::CTAS) blk_paged_attn_kernel(const 
         first = sched[8];
         cw.left = sched[16] - first;
         // Heads of a single tile each: every warp takes whole ones, in turn, and nothing is put together (495 requests of 5 tokens, 8 heads of 192,
-        // fp32, 36.7 -> 18.7 us; 503 of 1..16, 16 heads of 80, 62 -> 29).  Not with more than eight rows: these kernels lose 5 % where heads are longer
-        // for having both ways in them, the others 0 to 2 %.
+        // fp32, 36.7 -> 18.7 us; 503 of 1..16, 16 heads of 80, 62 -> 29).  Having both ways in them costs the kernels where heads
+        // are longer: nothing to 2 % for most (512 of 0..300 none; one request of 1000 7.37 -> 7.47), 4 % for 8 rows of 256 columns in fp32 (154.6 ->
+        // 160.6), 9 % for 6 requests of up to 5997, 2 rows of 80 columns, fp16 (13.6 -> 14.8).  With more than eight rows it was 5 %: not there.
         by_warps = GU <= 8 && !sched[14] && !sched[22] && sched[21] - sched[13] == cw.left;
         cw.r = (int)sched[9];
         if (cw.r + 1 < p.requests) cw.ahead = p.lengths[cw.r + 1];

@@ -177,3 +177,25 @@ def test_threads_give_what_one_call_gives(cuda_device):
 
     with ThreadPoolExecutor(4) as pool:
         assert list(pool.map(work, range(4))) == [30] * 4
+
+
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (F32, 64)])
+@pytest.mark.parametrize("requests", [513, 5000, 40000])
+def test_many_requests_of_a_few_tokens(cuda_device, dtype, d, requests):
+    """Tens of thousands of requests of 0..4 tokens on one page each, by the definition in 64 bits."""
+    g = torch.Generator("cuda").manual_seed(requests)
+    k, v = (torch.randn((requests + 3, 2, 4, d), generator=g, device="cuda").to(dtype) for _ in range(2))
+    q = torch.randn((requests, 4, d), generator=g, device="cuda").to(dtype)
+    table = torch.randperm(requests + 3, generator=g, device="cuda")[:requests].int()[:, None].contiguous()
+    n = torch.randint(0, 5, (requests,), generator=g, device="cuda").int()
+    out, lse = blockPagedAttention(q, k, v, table, n, d ** -0.5, return_lse=True)
+    a, b = (c[table[:, 0].long()].double().repeat_interleave(2, 1) for c in (k, v))
+    s = (a @ q.double()[..., None])[..., 0] * d ** -0.5
+    s.masked_fill_(torch.arange(4, device="cuda") >= n[:, None, None], -math.inf)
+    want = torch.nan_to_num(torch.softmax(s, -1))[:, :, None] @ b
+    log = torch.logsumexp(s, -1)
+    # (the tolerance of check(), with sums of at most 64 x 5 x 5 / 8 and values of at most 6)
+    w = 2 * (d + 2) * 2.0 ** -23 * 200 + 2.0 ** -17 + 200 * 2.0 ** -23
+    assert ((out.double() - want[:, :, 0]).abs() <= torch.finfo(dtype).eps / 2 * want[:, :, 0].abs() + 12 * w + 2.0 ** -25).all()
+    some = (n > 0)[:, None].expand_as(lse)
+    assert ((lse.double() - log)[some].abs() <= w + 2.0 ** -22 * 210).all() and (lse[~some] == -math.inf).all() and (out[n == 0] == 0).all()
